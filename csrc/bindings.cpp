@@ -90,6 +90,29 @@ std::vector<at::Tensor> invocation_gate_bwd(at::Tensor dout, at::Tensor pre, at:
 at::Tensor goldfish_mask(at::Tensor inputs, at::Tensor supervised, at::Tensor cu_seqlens, int64_t k,
                          int64_t context_width, int64_t seed, std::vector<int64_t> mix);
 int64_t embed_status(int64_t device);
+// kv_cache.cu
+at::Tensor cache_append(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cos, at::Tensor sin, at::Tensor pages,
+                        at::Tensor scales, at::Tensor table, at::Tensor lens, at::Tensor seqs, at::Tensor cu_new);
+at::Tensor cache_reserve(at::Tensor table, at::Tensor lens, at::Tensor refs, at::Tensor seqs, at::Tensor counts,
+                         int64_t page);
+void cache_free(at::Tensor table, at::Tensor lens, at::Tensor refs, at::Tensor seqs);
+at::Tensor cache_fork(at::Tensor pages, at::Tensor scales, at::Tensor table, at::Tensor lens, at::Tensor refs,
+                      at::Tensor src, at::Tensor dst);
+void cache_copy(at::Tensor pages, at::Tensor scales, at::Tensor src, at::Tensor dst);
+at::Tensor cache_compact(at::Tensor pages, at::Tensor scales, at::Tensor table, at::Tensor refs, at::Tensor out_pages,
+                         at::Tensor out_scales, at::Tensor out_table, at::Tensor out_refs);
+int64_t cache_status(int64_t device);
+// cache_attention.cu
+at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at::Tensor table, at::Tensor lens,
+                           at::Tensor seqs, at::Tensor cu_new, c10::optional<at::Tensor> prefix_lens,
+                           double softmax_scale, int64_t max_new);
+// logits.cu
+at::Tensor process_logits(at::Tensor logits, c10::optional<at::Tensor> tokens, c10::optional<at::Tensor> token_lens,
+                          c10::optional<at::Tensor> prompt_lens, c10::optional<at::Tensor> repetition,
+                          c10::optional<at::Tensor> presence, c10::optional<at::Tensor> frequency,
+                          c10::optional<at::Tensor> bias_offsets, c10::optional<at::Tensor> bias_ids,
+                          c10::optional<at::Tensor> bias_values, c10::optional<at::Tensor> allowed,
+                          c10::optional<at::Tensor> out);
 // gemm.cu
 at::Tensor gemm(at::Tensor a, bool a_mn, at::Tensor b, bool b_mn, c10::optional<at::Tensor> out,
                 c10::optional<at::Tensor> add, double alpha, double beta, int64_t bn, int64_t group_m,
@@ -159,4 +182,13 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("branch_write", &branch_write);
   m.def("branch_mix_bwd", &branch_mix_bwd);
   m.def("fmha_bwd", &fmha_bwd);
+  m.def("cache_append", &cache_append);
+  m.def("cache_reserve", &cache_reserve);
+  m.def("cache_free", &cache_free);
+  m.def("cache_fork", &cache_fork);
+  m.def("cache_copy", &cache_copy);
+  m.def("cache_compact", &cache_compact);
+  m.def("cache_status", &cache_status);
+  m.def("cache_attention", &cache_attention);
+  m.def("process_logits", &process_logits);
 }

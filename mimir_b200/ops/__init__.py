@@ -14,3 +14,6 @@ from mimir_b200.ops.moe import moe_plan  # noqa: F401
 from mimir_b200.ops.ngram import ngram_lookup  # noqa: F401
 from mimir_b200.ops.embedding import scaled_embedding  # noqa: F401
 from mimir_b200.ops.gemm import linear, swiglu_mlp, swiglu_mlp_supported  # noqa: F401
+from mimir_b200.ops.kv_cache import (  # noqa: F401
+    cache_append, cache_attention, cache_compact, cache_copy, cache_fork, cache_free, cache_reserve)
+from mimir_b200.ops.logits import process_logits  # noqa: F401

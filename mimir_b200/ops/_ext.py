@@ -14,7 +14,8 @@ _EXT = None
 _LOAD_ERROR: Exception | None = None
 
 # Kernel launches issued by one call of each binding (for launch accounting in benchmarks).
-_LAUNCHES_PER_CALL = {"fmha_status": 0, "fmha_plan": 1, "gemm_status": 0, "grouped_gemm_status": 0}
+_LAUNCHES_PER_CALL = {"fmha_status": 0, "fmha_plan": 1, "gemm_status": 0, "grouped_gemm_status": 0,
+                      "cache_status": 0, "cache_attention": 2, "cache_fork": 3, "cache_compact": 4}
 
 
 class _CountingModule:
@@ -79,21 +80,23 @@ def kernels_enabled(t: torch.Tensor | None = None) -> bool:
 
 class KernelTimeout(RuntimeError):
     """A hand-written kernel reported a launch whose outputs are not valid: a bounded wait ran out,
-    an expert-exchange route named a rank or row outside its buffers, or a token id was outside
-    the embedding table.  Raised by :func:`check_kernel_status`."""
+    an expert-exchange route named a rank or row outside its buffers, a token id was outside
+    the embedding table, or a key/value cache call named a slot, page or position that it does not
+    have.  Raised by :func:`check_kernel_status`."""
 
 
 def kernel_status(device: torch.device) -> dict:
     """Read and clear the status words of every kernel family on ``device``: the bounded-wait
     words of attention, dense GEMM and grouped GEMM (0: every wait since the last read completed),
-    the expert-exchange route word and the embedding's token-id word (0: every index in range)."""
+    the expert-exchange route word, the embedding's token-id word (0: every index in range) and
+    the key/value cache's word (0: every slot, page and length in range, every wait completed)."""
     if device.type != "cuda" or not available():
         return {}
     C = ext()
     index = device.index if device.index is not None else torch.cuda.current_device()
     return {"attention": int(C.fmha_status(device)), "gemm": int(C.gemm_status(index)),
             "grouped_gemm": int(C.grouped_gemm_status(index)), "moe_routes": int(C.moe_route_status(index)),
-            "embedding_ids": int(C.embed_status(index))}
+            "embedding_ids": int(C.embed_status(index)), "kv_cache": int(C.cache_status(index))}
 
 
 def check_kernel_status(device: torch.device, step=None) -> None:

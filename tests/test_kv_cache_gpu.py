@@ -1,0 +1,470 @@
+"""The kernels of the 8-bit paged key/value cache and of the logits operators against 64-bit formulas.
+
+Tolerances are derived, element by element, from the roundings that the kernels make (see
+``attention64``); bytes, scales, tables and counts have to be equal."""
+import math
+
+import pytest
+import torch
+
+from mimir_b200 import ops
+from mimir_b200.ops._ext import KernelTimeout, check_kernel_status, kernel_status
+from mimir_b200.ops.kv_cache import BLOCK, cache_append_reference, cache_values
+from mimir_b200.ops.logits import process_logits_reference
+
+from test_kv_cache import drive_pages, ints, pool, tables
+
+pytestmark = pytest.mark.gpu
+DIM = 128
+DEV = torch.device("cuda", 0)
+
+
+def on_gpu(st):
+    return {k: t.to(DEV) for k, t in st.items()}
+
+
+def filled(lens, kv, page, seed=0, spread=1.0, extra=3, first_page=0):
+    """A pool that holds ``lens`` tokens in each slot, pages in any order."""
+    gen = torch.Generator(DEV).manual_seed(seed)
+    need = [-(-n // page) for n in lens]
+    width = max(max(need), 1) + 1
+    pages = sum(need) + extra
+    x = torch.randn(pages, 2, kv, page // BLOCK, BLOCK, DIM, generator=gen, device=DEV)
+    e = torch.round(spread * torch.randn(pages, 2, kv, page // BLOCK, generator=gen, device=DEV)).to(torch.int32) - 7
+    st = dict(pages=(x * 100).clamp(-448, 448).to(torch.float8_e4m3fn).flatten(3, 4), scales=torch.ldexp(torch.ones_like(e, dtype=torch.float32), e),
+              table=torch.full((len(lens), width), -1, dtype=torch.int32, device=DEV), lens=ints(lens).to(DEV))
+    order = torch.randperm(pages, generator=gen, device=DEV).to(torch.int32).tolist()
+    for i, n in enumerate(need):
+        st["table"][i, :n] = ints([order.pop() for _ in range(n)]).to(DEV)
+    return st
+
+
+def attention64(q, st, seqs, counts, prefix=None, softmax_scale=DIM ** -0.5, p_bits=11):
+    """(64-bit attention, bound of the kernel's error), a sequence at a time.
+
+    The bound adds up: a score is a sum of 128 exact products in fp32 (its error at most 128 * 2^-24 of the sum of
+    their magnitudes, times two for the accumulator's own order, and as much again relative to the probability);
+    exp2 and the sums add under 2^-18; a probability is rounded to ``p_bits`` bits, or below fp16's normal
+    range, beside the largest product p * scale, to 2^-25 of it (the maximum may lag by 2^8 without loss,
+    it then lies higher in the range); the result is rounded to its type."""
+    kv = st["pages"].shape[2]
+    out = torch.zeros_like(q, dtype=torch.float64)
+    bound = torch.zeros_like(out)
+    unit = 2.0 ** -9 if q.dtype == torch.bfloat16 else 2.0 ** -12
+    row = 0
+    for i, (slot, count) in enumerate(zip(seqs, counts)):
+        n = int(st["lens"][slot])
+        if count and n:
+            k, v = cache_values(st["pages"], st["scales"], st["table"], slot, n).double()
+            pos = torch.arange(n - count, n, device=DEV)
+            limit = pos + 1 if prefix is None else torch.where(pos < prefix[i], torch.clamp_min(pos + 1, prefix[i]), pos + 1)
+            seen = torch.arange(n, device=DEV) < limit.clamp(0, n)[:, None]
+            x = q[row:row + count].double().unflatten(1, (kv, -1))
+            s = torch.einsum("tkgd,kjd->tkgj", x, k) * softmax_scale
+            off = torch.einsum("tkgd,kjd->tkgj", x.abs(), k.abs()) * softmax_scale * 2.0 ** -16
+            p = torch.softmax(s.masked_fill(~seen[:, None, None], -math.inf), -1)
+            p = torch.nan_to_num(p)  # a row that sees nothing
+            o = torch.einsum("tkgj,kjd->tkgd", p, v)
+            rel = 2 * off + 2.0 ** -18 + 2.0 ** -p_bits
+            err = torch.einsum("tkgj,kjd->tkgd", p * rel, v.abs()) + (p * (2 * off + 2.0 ** -18)).sum(-1)[..., None] * o.abs()
+            at = st["table"][slot, :-(-n // st["pages"].shape[3])].long()
+            size = st["scales"][at, 1].permute(1, 0, 2).flatten(1).double().repeat_interleave(BLOCK, 1)[:, :n]
+            most = (p * size[None, :, None]).amax(-1)[..., None]
+            err = err + 2.0 ** -25 * 448 * n * most
+            out[row:row + count] = o.flatten(1, 2)
+            bound[row:row + count] = (err + unit * (o.abs() + err)).flatten(1, 2)
+        row += count
+    return out, bound + 1e-30
+
+
+def check_attention(st, seqs, counts, heads, dtype=torch.bfloat16, prefix=None, seed=5, extra_rows=0, max_new=None, q=None,
+                    softmax_scale=None):
+    gen = torch.Generator(DEV).manual_seed(seed)
+    total = sum(counts)
+    if q is None:
+        q = (1.5 * torch.randn(total + extra_rows, heads, DIM, generator=gen, device=DEV)).to(dtype)
+    cu = ints([sum(counts[:i]) for i in range(len(counts) + 1)]).to(DEV)
+    out = ops.cache_attention(q, st["pages"], st["scales"], st["table"], st["lens"], ints(seqs).to(DEV), cu,
+                              None if prefix is None else ints(prefix).to(DEV), max_new=max_new, softmax_scale=softmax_scale)
+    ref, bound = attention64(q, st, seqs, counts, prefix, softmax_scale or DIM ** -0.5, p_bits=8)
+    check_kernel_status(DEV)
+    assert out.dtype == q.dtype and out.shape == q.shape and torch.isfinite(out).all()
+    err = (out.double() - ref).abs()
+    assert bool((err <= bound).all()), f"{(err / bound).max().item():.2f} of the bound"
+    assert not out[total:].any()
+    return q, out
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+def test_single_tokens_at_every_edge(page):
+    lens = [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 255, 257, 1000]
+    st = filled(lens, 2, page)
+    check_attention(st, list(range(len(lens))), [1] * len(lens), 8, max_new=1)
+    check_attention(st, list(range(len(lens)))[::-1], [1] * len(lens), 8)  # without the hint
+
+
+@pytest.mark.parametrize("heads,kv", [(1, 1), (3, 1), (5, 5), (8, 1), (16, 4), (12, 4), (24, 2), (20, 20)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_head_groups_and_types(heads, kv, dtype):
+    st = filled([70, 9, 300], kv, 32, seed=heads)
+    check_attention(st, [2, 0, 1], [1, 1, 1], heads, dtype, max_new=1)
+    check_attention(st, [2, 0, 1], [5, 70, 2], heads, dtype, max_new=70)
+
+
+@pytest.mark.parametrize("counts", [[2, 3, 1, 4], [0, 17, 0, 33], [64, 65, 1, 200], [300, 1, 129, 256]])
+@pytest.mark.parametrize("prefix", [None, "all", "half"])
+def test_several_tokens_and_prefixes(counts, prefix):
+    lens = [c + old for c, old in zip(counts, [5, 0, 700, 0])]
+    st = filled(lens, 2, 64, seed=sum(counts))
+    p = None if prefix is None else [n if prefix == "all" else n // 2 for n in lens]
+    check_attention(st, [0, 1, 2, 3], counts, 8, prefix=p, extra_rows=3)
+    check_attention(st, [0, 1, 2, 3], counts, 8, prefix=p, extra_rows=3, max_new=max(counts))
+
+
+def test_a_long_sequence_is_split_and_many_short_ones_are_not():
+    st = filled([40001], 1, 128)
+    check_attention(st, [0], [1], 4, max_new=1)
+    lens = [1 + i % 7 for i in range(1500)]  # more sequences than one launch takes
+    st = filled(lens, 1, 16)
+    check_attention(st, list(range(1500)), [1] * 1500, 2, max_new=1)
+
+
+def test_results_do_not_depend_on_the_run():
+    st = filled([5000, 77, 20000], 4, 64)
+    q, first = check_attention(st, [0, 1, 2], [1, 1, 1], 16, max_new=1)
+    for _ in range(5):
+        assert torch.equal(check_attention(st, [0, 1, 2], [1, 1, 1], 16, max_new=1, q=q)[1], first)
+
+
+def test_value_scales_far_apart():
+    """Blocks whose scales differ by 2^40: small weights of large values and large weights of small ones."""
+    st = filled([500, 33], 1, 16, spread=10.0)
+    st["scales"][:, 0] = 2.0 ** -7  # keys as usual
+    check_attention(st, [0, 1], [1, 1], 4, max_new=1)
+    check_attention(st, [0, 1], [40, 33], 4, max_new=40)
+
+
+def test_queries_of_any_size_and_a_scale_of_ones_own():
+    st = filled([200, 100], 2, 64)
+    gen = torch.Generator(DEV).manual_seed(1)
+    q = torch.randn(2, 8, DIM, generator=gen, device=DEV)
+    for factor, scale in ((2.0 ** 20, DIM ** -0.5 * 2.0 ** -20), (2.0 ** -30, DIM ** -0.5 * 2.0 ** 30), (1.0, 0.0)):
+        check_attention(st, [0, 1], [1, 1], 8, q=(q * factor).bfloat16(), softmax_scale=scale or 1e-9)
+
+
+def test_strided_queries():
+    st = filled([50, 90], 2, 32)
+    packed = torch.randn(9, 20, DIM, device=DEV).bfloat16()
+    check_attention(st, [0, 1], [4, 5], 8, q=packed[:, 7:15])
+    wide = torch.randn(8, 9, 2 * DIM, device=DEV).half().transpose(0, 1)
+    check_attention(st, [0, 1], [4, 5], 8, q=wide[..., :DIM])
+
+
+def test_bytes_beyond_the_length_do_not_matter():
+    """NaN bytes, NaN scales and pages of others behind a sequence's end, and in pages that it does not hold."""
+    for lens, counts in (([1, 17, 70], [1, 1, 1]), ([40, 150, 70], [33, 130, 2])):
+        st = filled(lens, 2, 64, seed=3)
+        q, want = check_attention(st, [0, 1, 2], counts, 8)
+        nan = torch.tensor(0x7F, dtype=torch.uint8, device=DEV)
+        held = torch.zeros(st["pages"].shape[0], dtype=torch.bool, device=DEV)
+        for i, n in enumerate(lens):
+            row = st["table"][i, :-(-n // 64)].long()
+            held[row] = True
+            inside = n - (len(row) - 1) * 64
+            st["pages"].view(torch.uint8)[row[-1], :, :, inside:] = nan
+            st["scales"][row[-1], :, :, -(-inside // BLOCK):] = math.nan
+        st["pages"].view(torch.uint8)[~held] = nan
+        st["scales"][~held] = math.nan
+        cu = ints([0, counts[0], sum(counts[:2]), sum(counts)]).to(DEV)
+        got = ops.cache_attention(q, st["pages"], st["scales"], st["table"], st["lens"], ints([0, 1, 2]).to(DEV), cu)
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("which", [0, 1])
+@pytest.mark.parametrize("count", [3, 60])
+def test_a_poisoned_block_reaches_the_rows_that_see_it(which, count):
+    n = 100
+    st = filled([n, 30], 2, 32)
+    q, want = check_attention(st, [0, 1], [count, 1], 8)
+    at = 98  # the block of tokens 96..99
+    st["scales"][st["table"][0, at // 32].long(), which, 1, at % 32 // BLOCK] = math.nan
+    got = ops.cache_attention(q, st["pages"], st["scales"], st["table"], st["lens"], ints([0, 1]).to(DEV),
+                              ints([0, count, count + 1]).to(DEV))
+    hit = torch.zeros(count + 1, 8, dtype=torch.bool, device=DEV)
+    hit[max(0, 96 - (n - count)):count, 4:] = True  # heads of the second key/value head, from position 96 on
+    assert torch.equal(torch.isnan(got).all(-1), hit) and torch.equal(torch.isnan(got).any(-1), hit)
+    assert torch.equal(got[~hit], want[~hit])
+
+
+def test_rows_without_keys_are_zero():
+    st = filled([10, 20], 1, 16)
+    st["lens"][0] = 0  # an emptied slot that is still asked for
+    q = torch.randn(4, 2, DIM, device=DEV).bfloat16()
+    out = ops.cache_attention(q, st["pages"], st["scales"], st["table"], st["lens"], ints([0, 1]).to(DEV),
+                              ints([0, 1, 2]).to(DEV))
+    assert not out[0].any() and out[1].any() and not out[2:].any()
+    with pytest.raises(KernelTimeout, match="kv_cache"):  # fewer tokens than new ones: reported
+        check_kernel_status(DEV)
+    empty = torch.zeros(0, dtype=torch.int32, device=DEV)
+    out = ops.cache_attention(q, st["pages"], st["scales"], st["table"], st["lens"], empty, ints([0]).to(DEV))
+    assert not out.any()
+
+
+def test_offsets_beyond_32_bits():
+    """Pages that lie more than 2^32 bytes into the pool."""
+    page, kv, pages = 256, 4, 17000  # 256 KB each: 4.4 GB
+    st = dict(pages=torch.zeros(pages, 2, kv, page, DIM, dtype=torch.float8_e4m3fn, device=DEV),
+              scales=torch.full((pages, 2, kv, page // BLOCK), 2.0 ** -7, device=DEV),
+              table=ints([[16999, 16990, 3]]).to(DEV), lens=ints([700]).to(DEV))
+    x = (100 * torch.randn(3, 2, kv, page, DIM, device=DEV, generator=torch.Generator(DEV).manual_seed(0))).clamp(-448, 448)
+    st["pages"].view(torch.uint8)[st["table"][0].long()] = x.to(torch.float8_e4m3fn).view(torch.uint8)
+    check_attention(st, [0], [1], 8, max_new=1)
+    check_attention(st, [0], [300], 8, max_new=300)
+    cos, sin = tables(1024, DIM)
+    k = torch.randn(700, kv, DIM, device=DEV).bfloat16()
+    ops.cache_append(k, k, k, cos.to(DEV), sin.to(DEV), st["pages"], st["scales"], st["table"], st["lens"],
+                     ints([0]).to(DEV), ints([0, 700]).to(DEV))
+    held = cache_values(st["pages"], st["scales"], st["table"], 0, 700)[1].transpose(0, 1)
+    assert bool(((held - k.float()).abs() <= k.float().abs() * 2.0 ** -4 + st["scales"].max() * 2.0 ** -10).all())
+    layers = st["pages"].view(2, pages // 2, 2, kv, page, DIM)
+    ops.cache_copy(layers, st["scales"].view(2, pages // 2, 2, kv, -1), ints([8499, -1]).to(DEV), ints([1, 2]).to(DEV))
+    assert torch.equal(layers[1, 1].view(torch.uint8), layers[1, 8499].view(torch.uint8)) and layers[1, 1].float().any()
+
+
+# ---------------------------------------------------------------------------------- append
+def append_both(st, q, k, v, seqs, cu, positions=2048):
+    """The kernel on the GPU and the formulation on the CPU, on the same state: equal, bit for bit."""
+    cos, sin = tables(positions, DIM)
+    host = {name: t.cpu() for name, t in st.items()}
+    want = cache_append_reference(q.cpu(), k.cpu(), v.cpu(), cos, sin, host["pages"], host["scales"], host["table"],
+                                  host["lens"], ints(seqs), ints(cu))
+    got = ops.cache_append(q, k, v, cos.to(DEV), sin.to(DEV), st["pages"], st["scales"], st["table"], st["lens"],
+                           ints(seqs).to(DEV), ints(cu).to(DEV))
+    check_kernel_status(DEV)
+    assert torch.equal(got.cpu(), want)
+    assert torch.equal(st["scales"].cpu().view(torch.int32), host["scales"].view(torch.int32))
+    assert torch.equal(st["pages"].cpu().view(torch.uint8), host["pages"].view(torch.uint8))
+    return got
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_append_writes_what_the_formula_says(page, dtype):
+    counts, old = [1, 5, 0, 16, 40, 1, 300], [0, 13, 9, 16, 3, 31, 1]
+    heads, kv = 6, 2
+    st = filled([c + o for c, o in zip(counts, old)], kv, page, spread=3.0)
+    gen = torch.Generator(DEV).manual_seed(4)
+    total = sum(counts) + 2  # two rows of no sequence
+    size = torch.exp(3 * torch.randn(total, 1, 1, generator=gen, device=DEV))
+    q, k, v = (torch.randn(total, h, DIM, generator=gen, device=DEV) for h in (heads, kv, kv))
+    k, v = k * size, v * size
+    v[:, :, 7] = 0
+    v[20:40] = 0  # whole blocks of zeros
+    cu = [sum(counts[:i]) for i in range(len(counts) + 1)]
+    got = append_both(st, q.to(dtype), k.to(dtype), v.to(dtype), list(range(len(counts))), cu)
+    assert not got[-2:].any()
+    # again: nothing changes
+    before = st["pages"].clone(), st["scales"].clone()
+    append_both(st, q.to(dtype), k.to(dtype), v.to(dtype), list(range(len(counts))), cu)
+    assert torch.equal(before[0].view(torch.uint8), st["pages"].view(torch.uint8)) and torch.equal(before[1], st["scales"])
+
+
+def test_append_of_many_tokens_and_packed_projections():
+    heads, kv, counts = 4, 2, [1900, 700, 3]
+    st = filled([c + 10 for c in counts], kv, 64)
+    packed = torch.randn(sum(counts), 2 * heads + 2 * kv, DIM, device=DEV).bfloat16()  # gate, q, k, v
+    cu = [0, 1900, 2600, 2603]
+    append_both(st, packed[:, heads:2 * heads], packed[:, 2 * heads:2 * heads + kv], packed[:, 2 * heads + kv:], [0, 1, 2], cu)
+
+
+def test_append_of_values_that_are_not_finite():
+    st = filled([33, 20], 2, 16)
+    x = torch.randn(23, 2, DIM, device=DEV).bfloat16()
+    k, v = x.clone(), x.clone()
+    k[3, 0, 5], v[9, 1, 100], v[22, 0, 0] = math.nan, math.inf, -math.inf
+    append_both(st, x, k, v, [0, 1], [0, 20, 23])
+    assert torch.isnan(st["scales"]).sum() == 3
+    st["lens"] += 1  # one more token into the poisoned block of the second sequence
+    st["table"][1, 1] = st["table"][1, 1].clamp_min(0)
+    append_both(st, x[:2], x[:2], x[:2], [1, 0], [0, 1, 2])
+
+
+def test_append_extremes():
+    """Zeros, the type's largest and smallest values, and a block that grows by 2^200."""
+    st = filled([48], 1, 16)
+    v = torch.zeros(48, 1, DIM, device=DEV)
+    v[0:16] = 1e-38
+    v[16, 0, 0], v[40] = 3e38, -3e38
+    append_both(st, v.bfloat16(), v.bfloat16(), v.bfloat16(), [0], [0, 48])
+    assert st["scales"][st["table"][0, 0].long(), 1, 0, 0] == 2.0 ** -32  # (keys of 3e38 rotate to infinities)
+    st["lens"][0] = 20
+    for new in (1e-12, 3e38):
+        st["lens"][0] += 1
+        append_both(st, v[:1].bfloat16(), v[:1].bfloat16(), torch.full((1, 1, DIM), new, device=DEV).bfloat16(), [0], [0, 1])
+
+
+# ---------------------------------------------------------------------------------- pages
+@pytest.mark.parametrize("seed,slots,width,pages,page", [(0, 6, 5, 20, 16), (1, 40, 30, 500, 64), (2, 16, 300, 3001, 32)])
+def test_page_operations_follow_the_model(seed, slots, width, pages, page):
+    drive_pages(DEV, slots, width, pages, page, steps=50, seed=seed)
+    check_kernel_status(DEV)
+
+
+def test_large_bookkeeping():
+    """More pages, sequences and entries than one step of the block takes."""
+    slots, width, pages = 2500, 40, 60000
+    table = torch.full((slots, width), -1, dtype=torch.int32, device=DEV)
+    lens, refs = torch.zeros(slots, dtype=torch.int32, device=DEV), torch.zeros(pages, dtype=torch.int32, device=DEV)
+    refs[::3] = 1  # held by others
+    counts = [1 + (37 * i) % 600 for i in range(slots)]
+    assert ops.cache_reserve(table, lens, refs, list(range(slots)), counts, 32).item() == 0
+    free, at = [p for p in range(pages) if p % 3], 0
+    host = table.tolist()
+    for i, c in enumerate(counts):
+        n = -(-c // 32)
+        assert host[i] == free[at:at + n] + [-1] * (width - n)
+        at += n
+    assert lens.tolist() == counts and refs.sum().item() == at + 20000
+    assert ops.cache_reserve(table, lens, refs, [0], [(width + 1) * 32], 32).item() == -1
+    lack = ops.cache_reserve(table, lens, refs, list(range(slots)), [600] * slots, 32).item()
+    need = sum(-(-(c + 600) // 32) - -(-c // 32) for c in counts)
+    assert lack == need - (pages - 20000 - at) and lens.tolist() == counts
+    ops.cache_free(table, lens, refs, list(range(0, slots, 2)))
+    assert refs.sum().item() == 20000 + sum(-(-c // 32) for c in counts[1::2]) and (table[::2] == -1).all()
+
+
+def test_bad_slots_and_pages_are_reported_and_skipped():
+    st = filled([40, 40], 1, 16)
+    st["table"][0, 1] = 10 ** 6
+    q = torch.randn(2, 2, DIM, device=DEV).bfloat16()
+    args = (st["pages"], st["scales"], st["table"], st["lens"], ints([0, 7]).to(DEV), ints([0, 1, 2]).to(DEV))
+    out = ops.cache_attention(q, *args)
+    assert torch.isfinite(out[1]).all() and kernel_status(DEV)["kv_cache"] in (1, 2)
+    cos, sin = (t.to(DEV) for t in tables(64, DIM))
+    before = st["pages"].clone()
+    st["lens"][0] = 17  # the bad page
+    ops.cache_append(q, q[:, :1], q[:, :1], cos, sin, *args)
+    assert kernel_status(DEV)["kv_cache"] in (1, 2) and torch.equal(before.view(torch.uint8), st["pages"].view(torch.uint8))
+    ops.cache_append(q, q[:, :1], q[:, :1], cos[:10], sin[:10], *args[:4], ints([1, 0]).to(DEV), args[5])
+    assert kernel_status(DEV)["kv_cache"] == 3  # positions that the tables do not have
+    refs = torch.ones(st["pages"].shape[0], dtype=torch.int32, device=DEV)
+    ops.cache_free(st["table"], st["lens"], refs, ints([9, -1, 0]).to(DEV))
+    assert kernel_status(DEV)["kv_cache"] in (1, 2)
+    assert kernel_status(DEV)["kv_cache"] == 0
+
+
+def test_refusals():
+    st = filled([20], 2, 16)
+    q, cu, seqs = torch.randn(1, 4, DIM, device=DEV).bfloat16(), ints([0, 1]).to(DEV), ints([0]).to(DEV)
+    rest = (st["table"], st["lens"], seqs, cu)
+
+    def attend(**kw):
+        a = dict(q=q, pages=st["pages"], scales=st["scales"]) | kw
+        return ops.cache_attention(a["q"], a["pages"], a["scales"], *kw.get("rest", rest))
+
+    for message, kw in (("divisible", dict(q=q[:, :3])), ("bfloat16 or float16", dict(q=q.float())),
+                        ("16-byte", dict(q=torch.randn(1, 4, DIM + 1, device=DEV).bfloat16()[..., 1:])),
+                        ("float8", dict(pages=st["pages"].view(torch.uint8))),
+                        ("scales", dict(scales=st["scales"].double())),
+                        ("contiguous", dict(pages=st["pages"][:, :, :, ::2])),
+                        ("int32", dict(rest=(st["table"].long(), *rest[1:]))),
+                        ("on cuda", dict(rest=(st["table"].cpu(), *rest[1:]))),
+                        ("one more entry", dict(rest=(*rest[:3], seqs)))):
+        with pytest.raises(ValueError, match=message):
+            attend(**kw)
+    k, (cos, sin) = q[:, :2], (t.to(DEV) for t in tables(64, DIM))
+    with pytest.raises(ValueError, match="as many tokens"):
+        ops.cache_append(q, k, k[:0], cos, sin, st["pages"], st["scales"], *rest)
+    with pytest.raises(ValueError, match="tables"):
+        ops.cache_append(q, k, k, cos.double(), sin, st["pages"], st["scales"], *rest)
+    with pytest.raises(ValueError, match="page_size"):
+        ops.cache_reserve(st["table"], st["lens"], st["lens"], seqs, seqs, 48)
+    with pytest.raises(ValueError, match="in place throughout"):
+        layers = (st["pages"][None], st["scales"][None])
+        refs = torch.zeros(st["pages"].shape[0], dtype=torch.int32, device=DEV)
+        ops.cache_compact(*layers, st["table"], refs, (*layers, st["table"].clone(), refs))
+    x = torch.randn(2, 40, device=DEV)
+    with pytest.raises(ValueError, match="need tokens"):
+        ops.process_logits(x, presence=torch.zeros(2, device=DEV))
+    with pytest.raises(ValueError, match="ceil"):
+        ops.process_logits(x, allowed=torch.zeros(2, 1, dtype=torch.int32, device=DEV))
+    with pytest.raises(ValueError, match="only where"):
+        y = torch.randn(2, 80, device=DEV)
+        ops.process_logits(y.view(2, 80)[:, :40], out=y.view(-1)[:80].view(2, 40))
+
+
+def test_calls_follow_the_current_stream():
+    """Everything of a decoding step on a side stream behind work that is still running there."""
+    st = filled([600, 130], 2, 64)
+    q = torch.randn(2, 8, DIM, device=DEV).bfloat16()
+    cu, seqs = ints([0, 1, 2]).to(DEV), ints([0, 1]).to(DEV)
+    cos, sin = (t.to(DEV) for t in tables(1024, DIM))
+    k = torch.randn(2, 2, DIM, device=DEV).bfloat16()
+    want = ops.cache_append(q, k, k, cos, sin, st["pages"], st["scales"], st["table"], st["lens"], seqs, cu)
+    want = ops.cache_attention(want, st["pages"], st["scales"], st["table"], st["lens"], seqs, cu)
+    big = torch.randn(4096, 4096, device=DEV)
+    late = torch.zeros_like(q)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            big = big @ big * 1e-3
+        late.copy_(q)
+        got = ops.cache_append(late, k, k, cos, sin, st["pages"], st["scales"], st["table"], st["lens"], seqs, cu)
+        got = ops.cache_attention(got, st["pages"], st["scales"], st["table"], st["lens"], seqs, cu)
+    side.synchronize()
+    assert torch.equal(got, want)
+
+
+def test_a_decoding_step_in_a_graph():
+    st = filled([600, 130], 2, 64)
+    q = torch.randn(2, 8, DIM, device=DEV).bfloat16()
+    cu, seqs = ints([0, 1, 2]).to(DEV), ints([0, 1]).to(DEV)
+    args = (st["pages"], st["scales"], st["table"], st["lens"], seqs, cu)
+    ops.cache_attention(q, *args)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = ops.cache_attention(q, *args)
+    for lens in ([600, 130], [3, 64], [64, 90]):
+        st["lens"].copy_(ints(lens))
+        q.copy_(torch.randn(2, 8, DIM))
+        graph.replay()
+        assert torch.equal(out, ops.cache_attention(q, *args))
+
+
+# ---------------------------------------------------------------------------------- logits
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,vocab", [(1, 1), (3, 31), (2, 4096), (5, 4097), (2, 10007), (7, 32768)])
+def test_logits_against_the_rules(rows, vocab, dtype):
+    gen = torch.Generator(DEV).manual_seed(vocab)
+    x = (3 * torch.randn(rows, vocab + 8, generator=gen, device=DEV)).to(dtype)[:, :vocab]  # rows with a stride
+    x[0, 0] = math.inf
+    x[-1, -1] = math.nan
+    most = 90
+    tokens = torch.randint(-2, min(vocab + 2, 40), (rows, most), generator=gen, device=DEV).to(torch.int32)
+    lens = torch.randint(0, most + 1, (rows,), generator=gen, device=DEV).to(torch.int32)
+    prompt = lens // 2
+    rep, pres, freq = (torch.rand(rows, generator=gen, device=DEV) + a for a in (0.5, 0.0, -0.5))
+    offsets = ints([0] + [40] * (rows - 1) + [67]).to(DEV) if rows > 1 else ints([3, 67]).to(DEV)
+    ids = torch.randint(-1, min(vocab + 1, 9), (67,), generator=gen, device=DEV).to(torch.int32)  # many equal ones
+    values = torch.randn(67, generator=gen, device=DEV)
+    allowed = torch.randint(-2 ** 31, 2 ** 31, (rows, -(-vocab // 32)), generator=gen, device=DEV).to(torch.int32)
+    kw = dict(tokens=tokens, token_lens=lens, prompt_lens=prompt, repetition=rep, presence=pres, frequency=freq,
+              bias=(offsets, ids, values), allowed=allowed)
+    for drop in ([], ["allowed"], ["bias"], ["presence", "frequency"], ["repetition"], ["token_lens", "prompt_lens"],
+                 ["tokens", "token_lens", "prompt_lens", "repetition", "presence", "frequency"]):
+        some = {k: v for k, v in kw.items() if k not in drop}
+        got = ops.process_logits(x, **some)
+        b = some.get("bias", (None, None, None))
+        ref = process_logits_reference(x.double(), *(some.get(k) for k in (
+            "tokens", "token_lens", "prompt_lens", "repetition", "presence", "frequency")), *b, some.get("allowed"))
+        assert got.dtype == torch.float32
+        # at most: a quotient, four sums and up to 67 biases, each rounded to 2^-24 of sizes under 2^8
+        torch.testing.assert_close(got, ref.float(), rtol=2.0 ** -21, atol=72 * 2.0 ** -24 * 2.0 ** 8, equal_nan=True)
+        assert torch.equal(got, ops.process_logits(x, **some)) or torch.isnan(got).any()
+    if dtype == torch.float32:
+        y = x.contiguous()
+        want = ops.process_logits(y, **kw)
+        assert ops.process_logits(y, **kw, out=y) is not None
+        torch.testing.assert_close(y, want, rtol=0, atol=0, equal_nan=True)
