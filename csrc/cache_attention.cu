@@ -11,71 +11,71 @@
 // tokens, so that a key is read once for all of them.  A producer warp brings 64 keys and values
 // (8 KB each) a stage by TMA with the 128-byte swizzle; four warps take 16 keys each, with a
 // softmax of their own, and join at the end of a segment.  A segment that spans blocks leaves partial
-// sums, which a second kernel joins in the order of the keys (no atomics: results do not depend on
-// scheduling).
+// sums, and the last of its blocks to finish joins them in the order of the keys (so that results do
+// not depend on which block that is).
 //
-// Matrix products are m16n8k16 with fp16 operands and fp32 sums.  Bytes become fp16 exactly; the
-// scales, powers of two, stay outside: a key block's multiplies its scores, a value block's enters
-// the exponent of the probability that multiplies the values, exp2(x + ev - M) with a maximum M of
-// x + ev of its own (so it neither overflows nor loses small weights), beside exp2(x - m) for the
-// sum.  Probabilities are rounded to fp16 (11 bits) for the product.  Query rows are shifted by a
-// power of two into fp16's range, so that bf16 rows keep all their bits.
+// Matrix products are m16n8k16 with fp16 operands and fp32 sums, keys or head dimensions as the 16 and
+// query rows as the 8 columns: a group's few rows fill the narrow side.  Bytes become fp16
+// exactly; the scales, powers of two, stay outside: a key block's multiplies its scores, a value
+// block's enters the exponent of the probability that multiplies the values, exp2(x + ev - M) with a
+// maximum M of x + ev of its own (so it neither overflows nor loses small weights), beside exp2(x - m)
+// for the sum.  Probabilities are rounded to fp16 (11 bits) for the product.  Query rows are shifted by
+// a power of two into fp16's range, so that bf16 rows keep all their bits.
 // The contraction over the head dimension may run in any order: thread c of a quad takes the bytes
 // 32c..32c+31 of a key row, which two 16-byte loads bring without bank conflicts under the swizzle, and
-// the same dimensions of the query rows.  Of the values it takes 16 bytes of four rows; output column
-// 16 g + j belongs to column g of product j.
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
+// the same dimensions of the query rows.  Of the values thread (g, c) takes the bytes 16g..16g+15 of
+// four rows; row g of product j is dimension 16g + 2j, row g + 8 the one after it.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
+
 #include "common.cuh"
-#include "kv_cache.cuh"
-#include "tma.cuh"
+#include "serving.h"
 
 using namespace mimir;
 
 namespace {
 
-constexpr int kKeys = 64;                      // keys of a unit
-constexpr int kStages = 4;
+constexpr int kKeys = kAttentionKeys;          // keys of a unit
 constexpr int kWarps = 4;                      // consumers
 constexpr int kThreads = (kWarps + 1) * 32;
-constexpr int kRows = 16;                      // rows of a tile
+constexpr int kRows = kAttentionRows;          // rows of a tile
 constexpr uint32_t kHalfStage = kKeys * kCacheDim;
 constexpr uint32_t kStageBytes = 2 * kHalfStage;
-constexpr int kMaxSeqs = 1024;                 // sequences of one launch
 constexpr int kOutLd = 132;                    // floats of a row in the join buffer
+constexpr int kQueryLd = 272;                  // bytes of a query row in shared memory: 16 spread over the banks
+constexpr int kWindow = 32;                    // sequences whose lengths a block keeps at hand
 constexpr float kLowest = -3e38f;
 constexpr float kGrowth = 8.f;                 // maxima move only when they grow by more than 2^8
+constexpr int kEnds = kAttentionEnds;
 
-struct Params {
-  const void* q;
-  int64_t q_tok, q_head;
-  void* out;                                   // [tokens, H, 128]
-  const float* scales;
-  const int *table, *lens, *seqs, *cu, *prefix;
-  int slots, width, n, tokens, H, KV, group, page, page_shift, npages;
-  float scale_log2;
-  int4* desc;                                  // per block: the segment that it begins and others finish
-  float* parts;                                // [blocks][2][16][128]
-  float2* part_ml;                             // [blocks][2][16]: maximum and sum
-  int last_batch;
-  int* status;
+using Params = AttentionParams;
+
+// kTiles: products' widths of 8 that hold the tile's rows.  Eight rows leave registers and shared
+// memory for three blocks an SM, sixteen for two.
+template <int kTiles>
+struct Shape {
+  static constexpr int kRowsHeld = 8 * kTiles;
+  static constexpr int kStages = kTiles == 1 ? 3 : 4;
+  static constexpr int kBlocksPerSm = kTiles == 1 ? 3 : 2;
 };
 
+template <int kStages>
 struct __align__(8) Barriers {
   uint64_t full[kStages];
   uint64_t empty[kStages];
+  uint64_t q_full[2];
+  uint64_t q_empty[2];
 };
 
-struct Seq {
-  int len, row, count, slot;  // tokens, first new row, new rows, page table row
+struct __align__(8) Seq {
+  int len, row, count, slot, prefix, pad;  // tokens, first new row, new rows, page table row
 };
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -89,6 +89,11 @@ __device__ __forceinline__ uint32_t f16_of_lo(uint32_t w) {  // bytes 0, 1 of w 
 __device__ __forceinline__ uint32_t f16_of_hi(uint32_t w) {  // bytes 2, 3
   uint32_t r;
   asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t w) {  // 16-bit values: row g, columns 2c, 2c + 1 a thread
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(w));
   return r;
 }
 __device__ __forceinline__ uint4 lds128(uint32_t addr) {
@@ -123,69 +128,153 @@ struct Pair<__half> {
 };
 
 // Keys that the row of token `tok` (of s.count new ones) sees.
-__device__ __forceinline__ int row_limit(const Seq& s, int prefix, int tok) {
+__device__ __forceinline__ int row_limit(const Seq& s, int tok) {
   const int pos = s.len - s.count + tok;
   int lim = pos + 1;
-  if (pos < prefix) lim = max(lim, prefix);
+  if (pos < s.prefix) lim = max(lim, s.prefix);
   return max(min(lim, s.len), 0);
 }
 
-// A share of the line of units, one segment at a time.
-struct Walk {
-  const int64_t* first;  // units before a sequence
-  const Seq* seqs;
-  int n, KV, group;
-  int64_t u, end;
-  int i;
-  // the segment
-  int h, rt, t0, t1, tiles;
-  int64_t seg_begin;
-  __device__ void start() {
-    int lo = 0, hi = n - 1;  // the last sequence with first <= u (empty ones have no units)
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (first[mid] <= u) lo = mid;
-      else hi = mid - 1;
+// A part of a segment: tiles t0 .. t1 - 1 of sequence i, head h, row tile rt.
+struct Segment {
+  int i, h, rt, t0, t1, tiles;
+  int64_t first_tile;  // where its tiles start on the line
+};
+
+// Sequence i of the batch; a bad slot or length is reported and read as no tokens.
+__device__ Seq load_seq(const Params& p, int i) {
+  Seq s;
+  s.row = p.cu[i];
+  s.count = max(min(p.cu[i + 1], p.tokens) - s.row, 0);
+  if (s.row < 0) s.count = 0;
+  s.slot = p.seqs[i];
+  s.prefix = p.prefix != nullptr ? p.prefix[i] : 0;
+  s.len = 0;
+  if (s.slot < 0 || s.slot >= p.slots) {
+    s.slot = 0;
+    if (s.count > 0) record_status(p.status, kCacheBadSlot);
+  } else {
+    s.len = p.lens[s.slot];
+    if (s.len < s.count) record_status(p.status, kCacheBadLength);
+    if (s.len < 0) s.len = 0;
+    if (s.len > p.width * p.page) {
+      s.len = p.width * p.page;
+      record_status(p.status, kCacheBadPage);
     }
-    i = lo;
   }
-  __device__ bool next() {
-    if (u >= end) return false;
-    while (first[i + 1] <= u) ++i;
-    const Seq& s = seqs[i];
-    const int rts = (s.count * group + kRows - 1) / kRows;
-    tiles = max((s.len + kKeys - 1) / kKeys, 1);
-    const int64_t local = u - first[i];
-    const int64_t seg = local / tiles;
-    t0 = (int)(local % tiles);
-    h = (int)(seg / rts);
-    rt = (int)(seg % rts);
-    seg_begin = u - t0;
-    t1 = (int)min((int64_t)tiles, t0 + (end - u));
-    u += t1 - t0;
-    return true;
+  return s;
+}
+__device__ __forceinline__ int seq_tiles(const Seq& s) { return max((s.len + kKeys - 1) / kKeys, 1); }
+__device__ __forceinline__ int seq_row_tiles(const Params& p, const Seq& s) {
+  return (s.count * p.group + kRows - 1) / kRows;
+}
+__device__ __forceinline__ int64_t seq_units(const Params& p, const Seq& s) {
+  return (int64_t)p.KV * seq_row_tiles(p, s) * (seq_tiles(s) + kEnds);
+}
+
+// A block's share of the line, one segment at a time.
+struct Walk {
+  const Params& p;
+  const Seq* window;   // sequences from `from` on: what a block's share meets, as a rule
+  int from, i;         // i: the sequence at u, which starts at `base`
+  int64_t base, u, end;
+  Seq s;
+  __device__ Seq seq(int x) const { return x - from < kWindow ? window[x - from] : load_seq(p, x); }
+  __device__ bool next(Segment& g) {
+    while (u < end) {
+      int64_t units;
+      while (base + (units = seq_units(p, s)) <= u) {
+        base += units;
+        s = seq(++i);
+      }
+      const int rts = seq_row_tiles(p, s);
+      g.i = i;
+      g.tiles = seq_tiles(s);
+      const int length = g.tiles + kEnds;
+      const int64_t local = u - base;
+      int off;
+      if (local >> 32) {
+        const int64_t seg = local / length;
+        off = (int)(local - seg * length);
+        g.h = (int)(seg / rts);
+        g.rt = (int)(seg % rts);
+      } else {
+        const uint32_t x = (uint32_t)local / (uint32_t)length;
+        off = (int)((uint32_t)local - x * (uint32_t)length);
+        g.h = (int)(x / (uint32_t)rts);
+        g.rt = (int)(x % (uint32_t)rts);
+      }
+      const int stop = (int)min((int64_t)length, off + (end - u));
+      g.first_tile = u - off + kEnds;
+      g.t0 = max(off - kEnds, 0);
+      g.t1 = max(stop - kEnds, 0);
+      u += stop - off;
+      if (g.t1 > g.t0) return true;
+    }
+    return false;
   }
 };
 
-template <typename T, bool kFull>
-__global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
+// Joins the parts of a segment, blocks b0 .. b1: a warp a row, a lane four columns.
+template <typename T>
+__device__ void join_parts(const Params& p, const Segment& sg, const Seq& s, int rows, int b0, int b1, int warp, int lane) {
+  auto part_of = [&](int b) { return (int64_t)b * 2 + (b == b0 ? 1 : 0); };
+  for (int r = warp; r < rows; r += kWarps) {
+    float m = kLowest, sum = 0.f;
+    for (int b = b0 + lane; b <= b1; b += 32) m = fmaxf(m, __ldcg(&p.part_ml[part_of(b) * kRows + r]).x);
+    m = warp_max(m);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int base = b0; base <= b1; base += 32) {
+      float w = 0.f;
+      if (base + lane <= b1) {
+        const float2 ml = __ldcg(&p.part_ml[part_of(base + lane) * kRows + r]);
+        w = fast_exp2(ml.x - m);
+        sum += ml.y * w;
+      }
+      const int here = min(32, b1 - base + 1);
+#pragma unroll 8
+      for (int j = 0; j < here; ++j) {
+        const float f = __shfl_sync(0xffffffffu, w, j);
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(p.parts + (part_of(base + j) * kRows + r) * kCacheDim) + lane);
+        o.x += x.x * f, o.y += x.y * f, o.z += x.z * f, o.w += x.w * f;
+      }
+    }
+    sum = warp_sum(sum);
+    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
+    const int row = sg.rt * kRows + r;
+    T* dst = reinterpret_cast<T*>(p.out) + ((int64_t)(s.row + row / p.group) * p.H + sg.h * p.group + row % p.group) * kCacheDim;
+    reinterpret_cast<uint2*>(dst)[lane] = make_uint2(Pair<T>::put(o.x * inv, o.y * inv), Pair<T>::put(o.z * inv, o.w * inv));
+  }
+}
+
+template <typename T, int kTiles>
+__global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr int kMine = kFull ? 16 : 8;  // rows of a tile that can hold queries
+  constexpr int kMine = Shape<kTiles>::kRowsHeld;  // rows of a tile that can hold queries
+  constexpr int kStages = Shape<kTiles>::kStages;
   float* joined = reinterpret_cast<float*>(smem + kStages * kStageBytes);        // [kWarps][kMine][kOutLd]
   float* stats = joined + kWarps * kMine * kOutLd;                               // [kWarps][kMine][4]: m, M, l
   float* block_scales = stats + kWarps * kMine * 4;                              // [kStages][4 blocks][k, v]
-  Barriers* bar = reinterpret_cast<Barriers*>(block_scales + kStages * 8);
-  int64_t* first = reinterpret_cast<int64_t*>(bar + 1);                          // [n + 1]
-  Seq* seqs = reinterpret_cast<Seq*>(first + p.n + 1);                           // [n]
+  uint8_t* query_base = reinterpret_cast<uint8_t*>(block_scales + kStages * 8);  // [2][kMine][kQueryLd]
+  auto* bar = reinterpret_cast<Barriers<kStages>*>(query_base + 2 * kMine * kQueryLd);
+  Seq* window = reinterpret_cast<Seq*>(bar + 1);                                 // [kWindow]
+  // Units before a sequence, [n + 1]: needed until the stages are
+  int64_t* first = reinterpret_cast<int64_t*>(smem);
+  static_assert(sizeof(int64_t) * (kAttentionSeqs + 1) <= kStages * kStageBytes, "the line fits the stages");
   __shared__ int64_t scan_sums[kThreads / 32];
   __shared__ int64_t scan_base;
+  __shared__ int last_of[2];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&bar->full[s], 1 + 8);
       mbar_init(&bar->empty[s], kWarps);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bar->q_full[s], 32);
+      mbar_init(&bar->q_empty[s], kWarps);
     }
     fence_mbarrier_init();
     tma_prefetch_desc(&map);
@@ -194,29 +283,7 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
   // ---- the line of units
   for (int base = 0; base < p.n; base += kThreads) {
     const int i = base + (int)threadIdx.x;
-    int64_t units = 0;
-    if (i < p.n) {
-      Seq s;
-      s.row = p.cu[i];
-      s.count = max(min(p.cu[i + 1], p.tokens) - s.row, 0);
-      if (s.row < 0) s.count = 0;
-      s.slot = p.seqs[i];
-      s.len = 0;
-      if (s.slot < 0 || s.slot >= p.slots) {
-        s.slot = 0;
-        if (s.count > 0) record_status(p.status, kCacheBadSlot);
-      } else {
-        s.len = p.lens[s.slot];
-        if (s.len < s.count) record_status(p.status, kCacheBadLength);
-        if (s.len < 0) s.len = 0;
-        if (s.len > p.width * p.page) {
-          s.len = p.width * p.page;
-          record_status(p.status, kCacheBadPage);
-        }
-      }
-      seqs[i] = s;
-      units = (int64_t)p.KV * ((s.count * p.group + kRows - 1) / kRows) * max((s.len + kKeys - 1) / kKeys, 1);
-    }
+    const int64_t units = i < p.n ? seq_units(p, load_seq(p, i)) : 0;
     int64_t v = units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -232,12 +299,9 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
     if (threadIdx.x == kThreads - 1) scan_base = before + v;
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    first[p.n] = scan_base;
-    p.desc[blockIdx.x] = make_int4(-1, 0, 0, 0);
-  }
+  if (threadIdx.x == 0) first[p.n] = scan_base;
   __syncthreads();
-  const int64_t total = p.n > 0 ? first[p.n] : 0;
+  const int64_t total = first[p.n];
   // rows that belong to no sequence
   if (p.last_batch) {
     const int from = p.n > 0 ? min(max(p.cu[p.n], 0), p.tokens) : 0;
@@ -248,32 +312,52 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
   }
   const int64_t blocks = min((int64_t)gridDim.x, total);
   if (blockIdx.x >= blocks) return;
-  Walk walk{first, seqs, p.n, p.KV, p.group};
-  const int64_t u0 = total * blockIdx.x / blocks;
-  walk.u = u0;
-  walk.end = total * (blockIdx.x + 1) / blocks;
-  walk.start();
+  auto share = [&](int64_t b) {
+    return total < (1 << 22) ? (int64_t)((uint32_t)(total * b) / (uint32_t)blocks) : total * b / blocks;
+  };
+  Walk walk{p, window, 0, 0, 0, share(blockIdx.x), share(blockIdx.x + 1), Seq{}};
+  {
+    int lo = 0, hi = p.n - 1;  // the last sequence with first <= u (empty ones have no units)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (first[mid] <= walk.u) lo = mid;
+      else hi = mid - 1;
+    }
+    walk.from = walk.i = lo;
+    walk.base = first[lo];
+  }
+  if (threadIdx.x < kWindow && walk.from + (int)threadIdx.x < p.n) window[threadIdx.x] = load_seq(p, walk.from + threadIdx.x);
+  __syncthreads();
+  walk.s = window[0];
   const int piece = min(p.page, kKeys), pieces = kKeys / piece;  // keys that lie together, and their number in a unit
 
   // The tiles that a row tile needs: keys up to the largest limit of its rows.
-  auto tiles_needed = [&](const Seq& s, int prefix, int rt) {
-    const int last = min((rt * kRows + kRows - 1) / p.group, s.count - 1);
-    int lim = row_limit(s, prefix, last);
-    if (prefix > 0) lim = max(lim, row_limit(s, prefix, rt * kRows / p.group));
-    return (lim + kKeys - 1) / kKeys;
+  auto tiles_needed = [&](const Seq& s, int rt) {
+    return (row_limit(s, min((rt * kRows + kRows - 1) / p.group, s.count - 1)) + kKeys - 1) / kKeys;
   };
+  Segment sg;
 
   if (warp == kWarps) {
     // ------------------------------------------------------------ producer
     int it = 0;
     bool ok = true;
-    while (ok && walk.next()) {
-      const Seq s = seqs[walk.i];
-      const int prefix = p.prefix != nullptr ? p.prefix[walk.i] : 0;
-      const int t1 = min(walk.t1, tiles_needed(s, prefix, walk.rt));
+    for (int turn = 0; ok && walk.next(sg); ++turn) {
+      const Seq& s = walk.s;
+      // query rows of the tile, 16 bytes a lane, zeros beyond the last
+      if (turn >= 2 && !warp_wait(&bar->q_empty[turn & 1], ((turn >> 1) - 1) & 1, p.status, kCacheTimeout)) break;
+      for (int x = lane; x < kMine * 16; x += 32) {
+        const int r = sg.rt * kRows + (x >> 4), tok = r / p.group;
+        const bool held = tok < s.count;
+        const T* src = reinterpret_cast<const T*>(p.q);
+        if (held) src += (int64_t)(s.row + tok) * p.q_tok + (sg.h * p.group + r % p.group) * p.q_head + (x & 15) * 8;
+        const uint32_t dst = smem_u32(query_base + ((turn & 1) * kMine + (x >> 4)) * kQueryLd + (x & 15) * 16);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(held ? 16 : 0) : "memory");
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(&bar->q_full[turn & 1])) : "memory");
+      const int t1 = min(sg.t1, tiles_needed(s, sg.rt));
       const int* row = p.table + (int64_t)s.slot * p.width;
       int base = -32, mine = -1;  // page ids of the pieces base .. base + 31, one a lane
-      for (int t = walk.t0; ok && t < t1; ++t, ++it) {
+      for (int t = sg.t0; ok && t < t1; ++t, ++it) {
         const int st = it % kStages;
         if (t * pieces + pieces > base + 32) {
           base = t * pieces;
@@ -295,7 +379,7 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
         const int b = (lane >> 1) & 3;
         const int tok_b = t * kKeys + b * kCacheBlock;
         const int page_b = __shfl_sync(0xffffffffu, mine, (tok_b / piece - base) & 31);
-        const float* src = p.scales + (((int64_t)page_b * 2 + (lane & 1)) * p.KV + walk.h) * (p.page / kCacheBlock) +
+        const float* src = p.scales + (((int64_t)page_b * 2 + (lane & 1)) * p.KV + sg.h) * (p.page / kCacheBlock) +
                            (tok_b & (p.page - 1)) / kCacheBlock;
         if (lane < 8) {
           const uint32_t dst = smem_u32(block_scales + st * 8 + lane);
@@ -309,7 +393,7 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
           const int page = __shfl_sync(0xffffffffu, mine, t * pieces + x - base);
           if (lane < 2) {  // lane 0 the keys, lane 1 the values
             const uint32_t dst = smem_u32(smem + st * kStageBytes + lane * kHalfStage + x * piece * kCacheDim);
-            tma_load_3d(dst, &map, &bar->full[st], 0, (t * kKeys + x * piece) & (p.page - 1), (page * 2 + lane) * p.KV + walk.h);
+            tma_load_3d(dst, &map, &bar->full[st], 0, (t * kKeys + x * piece) & (p.page - 1), (page * 2 + lane) * p.KV + sg.h);
           }
           __syncwarp();
         }
@@ -325,31 +409,28 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
   const int g = lane >> 2, c = lane & 3;
   int it = 0;
   bool ok = true;
-  while (walk.next()) {
-    const Seq s = seqs[walk.i];
-    const int prefix = p.prefix != nullptr ? p.prefix[walk.i] : 0;
-    const int t1 = min(walk.t1, tiles_needed(s, prefix, walk.rt));
-    const int rows = min(s.count * p.group - walk.rt * kRows, kRows);
-    // query rows g and g + 8 of the tile: dimensions 32c .. 32c + 31
-    uint32_t qa[8][kFull ? 4 : 2];
-    float qs[kFull ? 2 : 1];
-    int lim[kFull ? 2 : 1];
+  Segment split[2];
+  int has_split = 0;
+  auto block_of = [&](int64_t unit) { return (int)(((unit + 1) * blocks - 1) / total); };
+  for (int turn = 0; walk.next(sg); ++turn) {
+    const Segment cur = sg;
+    if (ok) ok = warp_wait(&bar->q_full[turn & 1], (turn >> 1) & 1, p.status, kCacheTimeout);
+    const Seq s = walk.s;
+    const int t1 = min(cur.t1, tiles_needed(s, cur.rt));
+    const int rows = min(s.count * p.group - cur.rt * kRows, kRows);
+    // Rows 8n + g, dimensions 32c .. 32c + 31, as the products' second operand; and of rows
+    // 8n + 2c and 8n + 2c + 1, whose scores this thread gets, the factor and the limit.
+    uint32_t qb[kTiles][8][2];
+    float qs[kTiles][2];
+    int lim[kTiles][2];
     int min_lim = 0x7fffffff;
 #pragma unroll
-    for (int x = 0; x < (kFull ? 2 : 1); ++x) {
-      const int r = walk.rt * kRows + g + 8 * x;
-      const int tok = r / p.group, head = walk.h * p.group + r % p.group;
-      uint4 w[4] = {};
-      lim[x] = 0;
-      if (tok < s.count) {
-        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q) + (int64_t)(s.row + tok) * p.q_tok +
-                                                          head * p.q_head + 32 * c);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = src[i];
-        lim[x] = row_limit(s, prefix, tok);
-        min_lim = min(min_lim, lim[x]);
-      }
+    for (int n = 0; n < kTiles; ++n) {
       float top = 0.f;
+      uint4 w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        w[e] = lds128(smem_u32(query_base + ((turn & 1) * kMine + g + 8 * n) * kQueryLd + (4 * c + e) * 16));
       const uint32_t* ww = reinterpret_cast<const uint32_t*>(w);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
@@ -361,86 +442,112 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
       // the row's largest value to [2^13, 2^14): a power of two, nothing is rounded away
       const int shift = max(min(13 - ((__float_as_int(top) >> 23) - 127), 120), -115);
       const float f = __int_as_float((shift + 127) << 23);
-      qs[x] = p.scale_log2 * __int_as_float((127 - shift) << 23);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {  // word i: dimensions 32c + 2i, 2i + 1; step i / 2
         const float2 v = Pair<T>::get(ww[i]);
-        qa[i >> 1][(i & 1) * (kFull ? 2 : 1) + x] = half2_bits(v.x * f, v.y * f);
+        qb[n][i >> 1][i & 1] = half2_bits(v.x * f, v.y * f);
+      }
+      const float back = p.scale_log2 * __int_as_float((127 - shift) << 23);
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        qs[n][y] = __shfl_sync(0xffffffffu, back, (2 * c + y) * 4);
+        const int tok = (cur.rt * kRows + 8 * n + 2 * c + y) / p.group;
+        lim[n][y] = 0;
+        if (tok < s.count) {
+          lim[n][y] = row_limit(s, tok);
+          min_lim = min(min_lim, lim[n][y]);
+        }
       }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) min_lim = min(min_lim, __shfl_xor_sync(0xffffffffu, min_lim, o));
+    min_lim = __reduce_min_sync(0xffffffffu, min_lim);
+    if (lane == 0) mbar_arrive(&bar->q_empty[turn & 1]);
 
-    float acc[16][4];
+    float acc[kTiles][8][4];
+    float m[kTiles][2], M[kTiles][2], l[kTiles][2];
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
+    for (int n = 0; n < kTiles; ++n) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[j][e] = 0.f;
-    constexpr int R = kFull ? 2 : 1;
-    float m[R], M[R], l[R];
+      for (int j = 0; j < 8; ++j)
 #pragma unroll
-    for (int x = 0; x < R; ++x) m[x] = M[x] = kLowest, l[x] = 0.f;
+        for (int e = 0; e < 4; ++e) acc[n][j][e] = 0.f;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) m[n][y] = M[n][y] = kLowest, l[n][y] = 0.f;
+    }
 
-    for (int t = walk.t0; t < t1; ++t, ++it) {
+    for (int t = cur.t0; t < t1; ++t, ++it) {
       const int st = it % kStages;
       if (ok) ok = warp_wait(&bar->full[st], (it / kStages) & 1, p.status, kCacheTimeout);
       if (!ok) continue;
       const int key0 = t * kKeys + warp * kCacheBlock;
       if (key0 < s.len) {
         const uint32_t sk = smem_u32(smem + st * kStageBytes);
-        float sacc[2][4];
+        // scores of keys g and g + 8: two chains of sums, since a product waits for the one before it
+        float sacc[kTiles][2][4];
+        {
+          uint32_t kw[2][8];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
+          for (int y = 0; y < 2; ++y) {
+            const int row = warp * kCacheBlock + 8 * y + g;
+            const uint4 k0 = lds128(sk + row * 128 + (((2 * c) ^ (row & 7)) << 4));
+            const uint4 k1 = lds128(sk + row * 128 + (((2 * c + 1) ^ (row & 7)) << 4));
+            kw[y][0] = k0.x, kw[y][1] = k0.y, kw[y][2] = k0.z, kw[y][3] = k0.w;
+            kw[y][4] = k1.x, kw[y][5] = k1.y, kw[y][6] = k1.z, kw[y][7] = k1.w;
+          }
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sacc[nt][e] = 0.f;
-          const int row = warp * kCacheBlock + nt * 8 + g;
-          const uint4 k0 = lds128(sk + row * 128 + (((2 * c) ^ (row & 7)) << 4));
-          const uint4 k1 = lds128(sk + row * 128 + (((2 * c + 1) ^ (row & 7)) << 4));
-          const uint32_t kw[8] = {k0.x, k0.y, k0.z, k0.w, k1.x, k1.y, k1.z, k1.w};
+          for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            mma_f16(sacc[nt], qa[i][0], kFull ? qa[i][1] : 0u, qa[i][kFull ? 2 : 1], kFull ? qa[i][3] : 0u, f16_of_lo(kw[i]),
-                    f16_of_hi(kw[i]));
+            for (int e = 0; e < 4; ++e) sacc[n][0][e] = sacc[n][1][e] = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t a0 = f16_of_lo(kw[0][i]), a1 = f16_of_lo(kw[1][i]), a2 = f16_of_hi(kw[0][i]), a3 = f16_of_hi(kw[1][i]);
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) mma_f16(sacc[n][i & 1], a0, a1, a2, a3, qb[n][i][0], qb[n][i][1]);
+          }
         }
         const float ks = block_scales[st * 8 + warp * 2], vs = block_scales[st * 8 + warp * 2 + 1];
         // log2 of the values' scale; NaN stays NaN
         const float ev = vs == vs ? (float)((__float_as_int(vs) >> 23) - 127) : vs;
         const bool edge = key0 + kCacheBlock > min_lim;
-        float pw[R][4], pv[R][4];
+        float x[kTiles][4];  // keys g, g + 8 (e / 2), rows 2c, 2c + 1 (e % 2)
+        bool grown = false;
 #pragma unroll
-        for (int x = 0; x < R; ++x) {
-          const float f = qs[x] * ks;
-          float xs[4] = {sacc[0][2 * x] * f, sacc[0][2 * x + 1] * f, sacc[1][2 * x] * f, sacc[1][2 * x + 1] * f};
-          if (edge) {
-            const int rel = lim[x] - key0 - 2 * c;
-            xs[0] = rel > 0 ? xs[0] : -INFINITY;
-            xs[1] = rel > 1 ? xs[1] : -INFINITY;
-            xs[2] = rel > 8 ? xs[2] : -INFINITY;
-            xs[3] = rel > 9 ? xs[3] : -INFINITY;
-          }
-          float mx = fmaxf(fmaxf(xs[0], xs[1]), fmaxf(xs[2], xs[3]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const float my = mx + ev;
-          if (__any_sync(0xffffffffu, mx > m[x] + kGrowth || my > M[x] + kGrowth)) {
-            const float mn = fmaxf(m[x], mx), Mn = fmaxf(M[x], my);
-            l[x] *= fast_exp2(m[x] - mn);
-            const float a = fast_exp2(M[x] - Mn);
-            m[x] = mn, M[x] = Mn;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[j][2 * x] *= a, acc[j][2 * x + 1] *= a;
-          }
-          const float shift = ev - M[x];
+        for (int n = 0; n < kTiles; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            pw[x][e] = fast_exp2(xs[e] - m[x]);
-            pv[x][e] = fast_exp2(xs[e] + shift);
-            if (edge && xs[e] == -INFINITY) pv[x][e] = 0.f;  // also beside a poisoned block's NaN
-            l[x] += pw[x][e];
+            x[n][e] = (sacc[n][0][e] + sacc[n][1][e]) * (qs[n][e & 1] * ks);
+            if (edge && key0 + g + (e >> 1) * 8 >= lim[n][e & 1]) x[n][e] = -INFINITY;
+            grown = grown || x[n][e] > m[n][e & 1] + kGrowth || x[n][e] + ev > M[n][e & 1] + kGrowth;
           }
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n)
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              float mx = fmaxf(x[n][y], x[n][2 + y]);
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+              const float mn = fmaxf(m[n][y], mx), Mn = fmaxf(M[n][y], mx + ev);
+              l[n][y] *= fast_exp2(m[n][y] - mn);
+              const float f = fast_exp2(M[n][y] - Mn);
+              m[n][y] = mn, M[n][y] = Mn;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) acc[n][j][y] *= f, acc[n][j][2 + y] *= f;
+            }
         }
-        const uint32_t a0 = half2_bits(pv[0][0], pv[0][1]), a2 = half2_bits(pv[0][2], pv[0][3]);
-        const uint32_t a1 = kFull ? half2_bits(pv[R - 1][0], pv[R - 1][1]) : 0u, a3 = kFull ? half2_bits(pv[R - 1][2], pv[R - 1][3]) : 0u;
+        uint32_t pb[kTiles][2];
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) {
+          float pv[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            l[n][e & 1] += fast_exp2(x[n][e] - m[n][e & 1]);
+            pv[e] = fast_exp2(x[n][e] + (ev - M[n][e & 1]));
+            if (edge && x[n][e] == -INFINITY) pv[e] = 0.f;  // also beside a poisoned block's NaN
+          }
+          pb[n][0] = transpose_8x8(half2_bits(pv[0], pv[1]));
+          pb[n][1] = transpose_8x8(half2_bits(pv[2], pv[3]));
+        }
         const uint32_t sv = sk + kHalfStage;
         uint4 v[4];
 #pragma unroll
@@ -454,10 +561,13 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
           const uint32_t w0 = (&v[0].x)[q], w1 = (&v[1].x)[q], w2 = (&v[2].x)[q], w3 = (&v[3].x)[q];
           const uint32_t lo01 = __byte_perm(w0, w1, 0x5140), lo23 = __byte_perm(w2, w3, 0x5140);
           const uint32_t hi01 = __byte_perm(w0, w1, 0x7362), hi23 = __byte_perm(w2, w3, 0x7362);
-          mma_f16(acc[4 * q], a0, a1, a2, a3, f16_of_lo(lo01), f16_of_lo(lo23));
-          mma_f16(acc[4 * q + 1], a0, a1, a2, a3, f16_of_hi(lo01), f16_of_hi(lo23));
-          mma_f16(acc[4 * q + 2], a0, a1, a2, a3, f16_of_lo(hi01), f16_of_lo(hi23));
-          mma_f16(acc[4 * q + 3], a0, a1, a2, a3, f16_of_hi(hi01), f16_of_hi(hi23));
+          const uint32_t a0 = f16_of_lo(lo01), a1 = f16_of_hi(lo01), a2 = f16_of_lo(lo23), a3 = f16_of_hi(lo23);
+          const uint32_t b0 = f16_of_lo(hi01), b1 = f16_of_hi(hi01), b2 = f16_of_lo(hi23), b3 = f16_of_hi(hi23);
+#pragma unroll
+          for (int n = 0; n < kTiles; ++n) {
+            mma_f16(acc[n][2 * q], a0, a1, a2, a3, pb[n][0], pb[n][1]);
+            mma_f16(acc[n][2 * q + 1], b0, b1, b2, b3, pb[n][0], pb[n][1]);
+          }
         }
       }
       __syncwarp();
@@ -466,26 +576,23 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
 
     // ---- join the four warps
 #pragma unroll
-    for (int x = 0; x < R; ++x) {
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-      l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-      const int r = g + 8 * x;
-      float* o = joined + (warp * kMine + r) * kOutLd + 32 * c;
+    for (int n = 0; n < kTiles; ++n)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int q = (k + c) & 3;  // spreads the quad over the banks
+      for (int y = 0; y < 2; ++y) {
+        float sum = l[n][y];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        const int r = 8 * n + 2 * c + y;
+        float* o = joined + (warp * kMine + r) * kOutLd + 16 * g;
 #pragma unroll
-        for (int qq = 0; qq < 4; ++qq) {
-          if (qq != q) continue;
-          *reinterpret_cast<float4*>(o + 4 * qq) = make_float4(acc[4 * qq][2 * x], acc[4 * qq + 1][2 * x], acc[4 * qq + 2][2 * x], acc[4 * qq + 3][2 * x]);
-          *reinterpret_cast<float4*>(o + 16 + 4 * qq) = make_float4(acc[4 * qq][2 * x + 1], acc[4 * qq + 1][2 * x + 1], acc[4 * qq + 2][2 * x + 1], acc[4 * qq + 3][2 * x + 1]);
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<float4*>(o + 4 * q) = make_float4(acc[n][2 * q][y], acc[n][2 * q][2 + y], acc[n][2 * q + 1][y], acc[n][2 * q + 1][2 + y]);
+        if (g == 0) {
+          float* sp = stats + (warp * kMine + r) * 4;
+          sp[0] = m[n][y], sp[1] = M[n][y], sp[2] = sum;
         }
       }
-      if (c == 0) {
-        float* sp = stats + (warp * kMine + r) * 4;
-        sp[0] = m[x], sp[1] = M[x], sp[2] = l[x];
-      }
-    }
     asm volatile("bar.sync 1, 128;" ::: "memory");
     constexpr int kPer = kMine * kCacheDim / (kWarps * 32);  // values of a thread: 8 or 16, of one row
     const int r = threadIdx.x * kPer / kCacheDim, d0 = threadIdx.x * kPer % kCacheDim;
@@ -509,152 +616,82 @@ __global__ void __launch_bounds__(kThreads) cache_attention_kernel(const __grid_
           const float4 x = *reinterpret_cast<const float4*>(joined + (w * kMine + r) * kOutLd + d0 + e);
           o[e] += x.x * f[w], o[e + 1] += x.y * f[w], o[e + 2] += x.z * f[w], o[e + 3] += x.w * f[w];
         }
-      const bool begins = walk.t0 == 0, ends = walk.t1 == walk.tiles;
-      if (begins && ends) {
+      if (cur.t0 == 0 && cur.t1 == cur.tiles) {
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-        const int row = walk.rt * kRows + r;
+        const int row = cur.rt * kRows + r;
         uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) +
-                                              ((int64_t)(s.row + row / p.group) * p.H + walk.h * p.group + row % p.group) * kCacheDim + d0);
+                                              ((int64_t)(s.row + row / p.group) * p.H + cur.h * p.group + row % p.group) * kCacheDim + d0);
 #pragma unroll
         for (int e = 0; e < kPer; e += 8)
           dst[e / 8] = make_uint4(Pair<T>::put(o[e] * inv, o[e + 1] * inv), Pair<T>::put(o[e + 2] * inv, o[e + 3] * inv),
                                   Pair<T>::put(o[e + 4] * inv, o[e + 5] * inv), Pair<T>::put(o[e + 6] * inv, o[e + 7] * inv));
       } else {
-        const int64_t part = (int64_t)blockIdx.x * 2 + (begins ? 1 : 0);
+        const int64_t part = (int64_t)blockIdx.x * 2 + (cur.t0 == 0 ? 1 : 0);
         float4* dst = reinterpret_cast<float4*>(p.parts + (part * kRows + r) * kCacheDim + d0);
 #pragma unroll
         for (int e = 0; e < kPer; e += 4) dst[e / 4] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         if (d0 == 0) p.part_ml[part * kRows + r] = make_float2(mc, sum);
-        if (threadIdx.x == 0 && begins) {
-          // the block that holds the segment's last unit
-          const int64_t last = walk.seg_begin + walk.tiles - 1;
-          p.desc[blockIdx.x] = make_int4(walk.i, walk.h, walk.rt, (int)(((last + 1) * blocks - 1) / total));
-        }
       }
+    }
+    if (cur.t0 > 0 || cur.t1 < cur.tiles) {  // at most twice: the share's first segment and its last
+      split[cur.t0 == 0 ? 1 : 0] = cur;
+      has_split |= cur.t0 == 0 ? 2 : 1;
     }
     asm volatile("bar.sync 1, 128;" ::: "memory");  // the buffer is free again
   }
-}
-
-// Joins the partial sums of the segment that block `blockIdx.x` of the first kernel began.
-template <typename T>
-__global__ void __launch_bounds__(512) cache_attention_join_kernel(const Params p) {
-  const int4 d = p.desc[blockIdx.x];
-  if (d.x < 0) return;
-  const int first_row = p.cu[d.x], count = min(p.cu[d.x + 1], p.tokens) - first_row;
-  const int rows = min(count * p.group - d.z * kRows, kRows);
-  const int col = threadIdx.x & 127;
-  for (int r = threadIdx.x >> 7; r < rows; r += 4) {
-    float m = kLowest, sum = 0.f, o = 0.f;
-    for (int b = blockIdx.x; b <= d.w; ++b) {
-      const int64_t part = (int64_t)b * 2 + (b == (int)blockIdx.x ? 1 : 0);
-      const float2 ml = p.part_ml[part * kRows + r];
-      const float x = p.parts[(part * kRows + r) * kCacheDim + col];
-      const float mn = fmaxf(m, ml.x);
-      const float fa = fast_exp2(m - mn), fb = fast_exp2(ml.x - mn);
-      sum = sum * fa + ml.y * fb;
-      o = o * fa + x * fb;
-      m = mn;
-    }
-    const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    const int row = d.z * kRows + r;
-    T* dst = reinterpret_cast<T*>(p.out) + ((int64_t)(first_row + row / p.group) * p.H + d.y * p.group + row % p.group) * kCacheDim;
-    dst[col] = Pair<T>::one(o * inv);
+  if (!has_split) return;
+  // ---- The blocks of a segment lie side by side, from the one with its first tile to the one with its
+  // last.  Parts are announced once, at the end of the share; who comes last joins them.
+  __threadfence();
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+  if (threadIdx.x < 2 && (has_split >> threadIdx.x & 1)) {
+    const Segment& x = split[threadIdx.x];
+    const int b0 = block_of(x.first_tile), b1 = block_of(x.first_tile + x.tiles - 1);
+    const int before = atomicAdd(p.arrived + b0, 1);
+    last_of[threadIdx.x] = before == b1 - b0 ? b0 : -1;
+    if (before == b1 - b0) p.arrived[b0] = 0;
+  }
+  asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    if (!(has_split >> x & 1) || last_of[x] < 0) continue;
+    __threadfence();
+    const Seq s = walk.seq(split[x].i);
+    const int rows = min(s.count * p.group - split[x].rt * kRows, kRows);
+    join_parts<T>(p, split[x], s, rows, last_of[x], block_of(split[x].first_tile + split[x].tiles - 1), warp, lane);
   }
 }
 
-CUtensorMap pages_map(const at::Tensor& pages) {
-  const int64_t rows = pages.size(3), heads = pages.size(0) * 2 * pages.size(2);
-  bind_device_context();
-  CUtensorMap map;
-  cuuint64_t dims[3] = {(cuuint64_t)kCacheDim, (cuuint64_t)rows, (cuuint64_t)heads};
-  cuuint64_t strides[2] = {(cuuint64_t)kCacheDim, (cuuint64_t)(rows * kCacheDim)};
-  cuuint32_t box[3] = {(cuuint32_t)kCacheDim, (cuuint32_t)std::min<int64_t>(rows, kKeys), 1};
-  cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = tensor_map_encoder()(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, pages.data_ptr(), dims, strides, box, estr,
-                                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (pages) failed with code ", (int)r);
-  return map;
+template <int kTiles>
+constexpr size_t smem_bytes() {
+  using S = Shape<kTiles>;
+  return 1024 + S::kStages * kStageBytes + sizeof(float) * (kWarps * S::kRowsHeld * (kOutLd + 4) + S::kStages * 8) +
+         2 * S::kRowsHeld * kQueryLd + sizeof(Barriers<S::kStages>) + sizeof(Seq) * kWindow;
 }
 
-size_t smem_bytes(bool full, int n) {
-  const int mine = full ? 16 : 8;
-  return 1024 + kStages * kStageBytes + sizeof(float) * (kWarps * mine * (kOutLd + 4) + kStages * 8) + sizeof(Barriers) +
-         sizeof(int64_t) * (n + 1) + sizeof(Seq) * n;
-}
-
-template <typename T, bool kFull>
-void launch(const CUtensorMap& map, const Params& p, int grid) {
+template <typename T, int kTiles>
+cudaError_t launch(const CUtensorMap& map, const Params& p, int grid, cudaStream_t stream) {
   static bool set[64] = {false};
   int dev = 0;
-  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err != cudaSuccess) return err;
   if (!set[dev]) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(cache_attention_kernel<T, kFull>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        (int)smem_bytes(kFull, kMaxSeqs)));
+    err = cudaFuncSetAttribute(cache_attention_kernel<T, kTiles>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)smem_bytes<kTiles>());
+    if (err != cudaSuccess) return err;
     set[dev] = true;
   }
-  auto st = at::cuda::getCurrentCUDAStream();
-  cache_attention_kernel<T, kFull><<<grid, kThreads, smem_bytes(kFull, p.n), st>>>(map, p);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  cache_attention_join_kernel<T><<<grid, 512, 0, st>>>(p);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  grid = std::min(grid, Shape<kTiles>::kBlocksPerSm * 148);
+  cache_attention_kernel<T, kTiles><<<grid, kThreads, smem_bytes<kTiles>(), stream>>>(map, p);
+  return cudaGetLastError();
 }
 
 }  // namespace
 
-at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at::Tensor table, at::Tensor lens,
-                           at::Tensor seqs, at::Tensor cu_new, c10::optional<at::Tensor> prefix_lens,
-                           double softmax_scale, int64_t max_new) {
-  check_pool(pages, scales, 0);
-  const at::Device dev = pages.device();
-  check_rows(q, "q", dev);
-  check_batch(table, lens, seqs, cu_new, dev);
-  const int64_t H = q.size(1), KV = pages.size(2);
-  CACHE_CHECK(H >= 1 && H % KV == 0, "query heads ", H, " must be divisible by key/value heads ", KV);
-  CACHE_CHECK(q.size(0) * (H / KV) < (int64_t(1) << 31) - 64, "too many query rows");
-  CACHE_CHECK(table.size(1) * pages.size(3) < (int64_t(1) << 31) - 4096, "sequences of 2^31 tokens or more");
-  if (prefix_lens.has_value()) {
-    check_int32(*prefix_lens, "prefix_lens", 1, dev);
-    CACHE_CHECK(prefix_lens->size(0) == seqs.size(0), "prefix_lens needs one length for each of seqs");
-  }
-  c10::cuda::CUDAGuard guard(dev);
-  at::Tensor out = at::empty({q.size(0), H, kCacheDim}, q.options());
-  const int64_t n = seqs.size(0);
-  if (q.size(0) == 0) return out;
-  if (n == 0 || pages.size(0) == 0) return out.zero_();
-  const CUtensorMap map = pages_map(pages);
-  Params p{};
-  p.q = q.data_ptr();
-  p.q_tok = q.stride(0), p.q_head = q.stride(1);
-  p.out = out.data_ptr();
-  p.scales = scales.data_ptr<float>();
-  p.table = table.data_ptr<int>(), p.lens = lens.data_ptr<int>();
-  p.slots = (int)table.size(0), p.width = (int)table.size(1), p.tokens = (int)q.size(0);
-  p.H = (int)H, p.KV = (int)KV, p.group = (int)(H / KV);
-  p.page = (int)pages.size(3), p.page_shift = __builtin_ctz(p.page), p.npages = (int)pages.size(0);
-  p.scale_log2 = (float)(softmax_scale * 1.4426950408889634);
-  p.status = cache_status_word(dev);
-  const bool full = max_new < 1 || max_new * p.group > 8;
-  for (int64_t base = 0; base < n; base += kMaxSeqs) {
-    p.n = (int)std::min<int64_t>(kMaxSeqs, n - base);
-    p.seqs = seqs.data_ptr<int>() + base;
-    p.cu = cu_new.data_ptr<int>() + base;
-    p.prefix = prefix_lens.has_value() ? prefix_lens->data_ptr<int>() + base : nullptr;
-    p.last_batch = base + p.n == n;
-    // no more blocks than units: at most this many
-    const int64_t row_tiles = std::min<int64_t>(q.size(0), p.n) + q.size(0) * p.group / kRows + 1;
-    const int64_t most = row_tiles * KV * ((p.width * p.page + kKeys - 1) / kKeys + 1);
-    const int grid = (int)std::min<int64_t>(2 * 148, std::max<int64_t>(most, 1));
-    at::Tensor work = at::empty({grid * (int64_t)(4 + 2 * kRows * (kCacheDim + 2))}, q.options().dtype(at::kFloat));
-    float* w = work.data_ptr<float>();
-    p.desc = reinterpret_cast<int4*>(w);
-    p.parts = w + grid * 4;
-    p.part_ml = reinterpret_cast<float2*>(p.parts + (int64_t)grid * 2 * kRows * kCacheDim);
-    if (q.scalar_type() == at::kBFloat16)
-      full ? launch<__nv_bfloat16, true>(map, p, grid) : launch<__nv_bfloat16, false>(map, p, grid);
-    else
-      full ? launch<__half, true>(map, p, grid) : launch<__half, false>(map, p, grid);
-  }
-  return out;
+namespace mimir {
+cudaError_t launch_cache_attention(const CUtensorMap& map, const AttentionParams& p, bool bf16, bool full, int grid,
+                                   cudaStream_t stream) {
+  if (bf16) return full ? launch<__nv_bfloat16, 2>(map, p, grid, stream) : launch<__nv_bfloat16, 1>(map, p, grid, stream);
+  return full ? launch<__half, 2>(map, p, grid, stream) : launch<__half, 1>(map, p, grid, stream);
 }
+}  // namespace mimir

@@ -1,6 +1,6 @@
 // The 8-bit paged key/value cache: rotary + quantise + write (cache_append), and the bookkeeping
 // and movement of its pages (cache_reserve, cache_free, cache_fork, cache_compact, cache_copy).
-// Layout and status codes: kv_cache.cuh.
+// Layout and status codes: serving.h.
 //
 // Append.  A new token at position p gets x' = x * cos[p] + rot(x) * sin[p] (k and q; the two
 // products and their sum each rounded to fp32) and v' = v.  All new tokens of one head in one
@@ -9,16 +9,13 @@
 // held a smaller one, their bytes are rounded again to the new one.  Powers of two make every
 // product and quotient with a scale exact, so a value is rounded once (e4m3, nearest even), and
 // a token whose block later grows is rounded again only where it falls below the normal range.
-// One warp owns a (block, head, k or v): two tokens at a time, 16 lanes a token, each lane four
-// dimensions of either half, so that both partners of a rotation are in one thread and all
-// loads are 8 bytes a lane; the whole block stays in registers between the maximum and the write.
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
-#include "kv_cache.cuh"
+#include <algorithm>
+
+#include "serving.h"
 
 using namespace mimir;
 
@@ -28,14 +25,20 @@ __device__ int g_cache_status;
 
 __device__ __forceinline__ void report(int* status, int code) { atomicCAS(status, 0, code); }
 
-__device__ __forceinline__ float4 load4(const __nv_bfloat16* p) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
+template <typename T>
+__device__ __forceinline__ uint2 raw4(const T* p) {
+  return *reinterpret_cast<const uint2*>(p);
+}
+template <typename T>
+__device__ __forceinline__ float4 widen(uint2 w);
+template <>
+__device__ __forceinline__ float4 widen<__nv_bfloat16>(uint2 w) {
   const float2 a = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x));
   const float2 b = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
   return make_float4(a.x, a.y, b.x, b.y);
 }
-__device__ __forceinline__ float4 load4(const __half* p) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
+template <>
+__device__ __forceinline__ float4 widen<__half>(uint2 w) {
   const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&w.x));
   const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
   return make_float4(a.x, a.y, b.x, b.y);
@@ -57,10 +60,8 @@ __device__ __forceinline__ float turn(float x, float other, float c, float s) {
   return __fadd_rn(__fmul_rn(x, c), __fmul_rn(other, s));
 }
 
-// Rotates dimensions d..d+3 (lo) and d+64..d+67 (hi) of one head.
-__device__ __forceinline__ void rotate(float4& lo, float4& hi, const float* cos_row, const float* sin_row, int d) {
-  const float4 cl = *reinterpret_cast<const float4*>(cos_row + d), ch = *reinterpret_cast<const float4*>(cos_row + 64 + d);
-  const float4 sl = *reinterpret_cast<const float4*>(sin_row + d), sh = *reinterpret_cast<const float4*>(sin_row + 64 + d);
+// Rotates four dimensions d (lo) and their partners d + 64 (hi).
+__device__ __forceinline__ void rotate(float4& lo, float4& hi, float4 cl, float4 ch, float4 sl, float4 sh) {
   const float4 l = lo, h = hi;
   lo = make_float4(turn(l.x, -h.x, cl.x, sl.x), turn(l.y, -h.y, cl.y, sl.y), turn(l.z, -h.z, cl.z, sl.z),
                    turn(l.w, -h.w, cl.w, sl.w));
@@ -90,219 +91,221 @@ __device__ __forceinline__ float4 from_e4m3(uint32_t w) {
 }
 __device__ __forceinline__ float4 times(float4 v, float f) { return make_float4(v.x * f, v.y * f, v.z * f, v.w * f); }
 
-// A value that is not finite becomes zero and is reported in `bad`.
-__device__ __forceinline__ void take_finite(float4& v, float& amax, bool& bad) {
+// The largest magnitude, as bits; a value that is not finite becomes zero and is reported in `bad`.
+__device__ __forceinline__ uint32_t take_finite(float4& v, bool& bad) {
   float* x = reinterpret_cast<float*>(&v);
+  uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     if (!(fabsf(x[i]) <= 3.402823466e38f)) {
       x[i] = 0.f;
       bad = true;
     }
-    amax = fmaxf(amax, fabsf(x[i]));
+    top = max(top, __float_as_uint(fabsf(x[i])));
   }
+  return top;
 }
 
 constexpr int kAppendThreads = 256;
-constexpr int kMaxChunk = 16;
+constexpr int kTeams = kAppendThreads / 16;  // a team of 16 lanes holds one row of a head
+constexpr int kHeads = 4;                    // key/value heads of a thread block
 
+// One block of 16 cached tokens (those of its tokens that are new) and up to four key/value heads with
+// their query heads.  Thread block b finds its tokens itself: sequence i has at most
+// new / 16 + 2 blocks, so the ones from cu[i] / 16 + 3 i on are its own, and a few stay empty.  After that
+// all loads are under way at once.  A team's items are dealt rows first: sixteen rows give every
+// team a row and all its heads, one row gives every team a head.
 template <typename T>
-struct AppendParams {
-  const T *q, *k, *v;
-  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;  // strides in elements
-  T* q_out;                                             // [tokens, H, 128]
-  const float *cos, *sin;
-  int64_t positions;
-  uint8_t* pages;
-  float* scales;
-  int64_t npages;
-  const int *table, *lens, *seqs, *cu;
-  int slots, width, n, tokens, H, KV, page, chunk;
-  int* status;
-};
-
-struct TokenInfo {
-  int pos;     // -1: no position (the row belongs to no sequence, or its slot or length is bad)
-  int page;    // -1: nothing is written
-  int count;   // tokens of its block that it leads (0: another token leads)
-};
-
-// blockIdx.x: `chunk` rows of the new tokens; blockIdx.y: a key/value head and its query heads.
-template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) cache_append_kernel(const AppendParams<T> p) {
-  __shared__ TokenInfo info[kMaxChunk];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int t0 = blockIdx.x * p.chunk;
-  const int here = min(p.chunk, p.tokens - t0);
-  for (int r = warp; r < here; r += kAppendThreads / 32) {
-    const int t = t0 + r;
-    // the last i with cu[i] <= t, 32 candidates a step
-    int lo = 0, size = p.n + 1;
+__global__ void __launch_bounds__(kAppendThreads, 3) cache_append_kernel(const AppendParams p) {
+  __shared__ int at_row, at_pos, at_page, at_rows, at_written;  // first new row, its position, page, rows, rows written
+  __shared__ uint32_t tops[kHeads][2];                          // largest magnitude, keys and values
+  __shared__ int exponents[kHeads][2], poisoned[kHeads][2];
+  const int lane = threadIdx.x & 31, team = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4;
+  if (threadIdx.x < 32) {
+    const int b = blockIdx.x;
+    int lo = 0, size = p.n + 1;  // the last i with cu[i] / 16 + 3 i <= b, 32 candidates a step
     while (size > 1) {
       const int step = (size + 31) / 32;
-      const int at = lo + lane * step;
-      const int c = __popc(__ballot_sync(0xffffffffu, at < lo + size && p.cu[min(at, p.n)] <= t));
+      const int at = min(lo + lane * step, p.n);
+      const int c = __popc(__ballot_sync(0xffffffffu, lo + lane * step < lo + size && p.cu[at] / kCacheBlock + 3 * at <= b));
       const int next = lo + max(c - 1, 0) * step;
       size = min(step, lo + size - next);
       lo = next;
     }
     if (lane == 0) {
-      TokenInfo ti{-1, -1, 0};
+      int rows = 0, written = 0, row = 0, pos = 0, page = -1;
       if (lo < p.n) {
-        const int first = p.cu[lo], end = min(p.cu[lo + 1], p.tokens), slot = p.seqs[lo];
-        if (t < first || slot < 0 || slot >= p.slots) {
-          report(p.status, kCacheBadSlot);
-        } else {
-          const int start = p.lens[slot] - (p.cu[lo + 1] - first);
-          const int pos = start + t - first;
-          if (start < 0 || pos >= p.positions) {
-            report(p.status, kCacheBadLength);
-          } else {
-            ti.pos = pos;
-            const int j = pos / p.page;
-            const int page = j < p.width ? p.table[(int64_t)slot * p.width + j] : -1;
-            if (page < 0 || page >= p.npages) report(p.status, kCacheBadPage);
-            else ti.page = page;
-            if (t == first || pos % kCacheBlock == 0)
-              ti.count = min(min(kCacheBlock - pos % kCacheBlock, end - t), (int)p.positions - pos);
+        const int first = p.cu[lo], stop = min(p.cu[lo + 1], p.tokens), slot = p.seqs[lo];
+        const int j = b - (first / kCacheBlock + 3 * lo), count = max(stop - first, 0);
+        const bool good = slot >= 0 && slot < p.slots;
+        const int start = good ? p.lens[slot] - (p.cu[lo + 1] - first) : 0;
+        if (first >= 0 && good && start >= 0) {
+          const int64_t block = (int64_t)(start / kCacheBlock + j) * kCacheBlock;
+          const int64_t from = max(block, (int64_t)start), to = min(block + kCacheBlock, (int64_t)start + count);
+          rows = (int)max(to - from, (int64_t)0);
+          pos = (int)from;
+          row = first + pos - start;
+          written = (int)min(max(p.positions - from, (int64_t)0), (int64_t)rows);
+          if (written < rows) report(p.status, kCacheBadLength);
+          if (rows > 0) {
+            const int x = pos / p.page;
+            page = x < p.width ? p.table[(int64_t)slot * p.width + x] : -1;
+            if (page < 0 || page >= p.npages) {
+              report(p.status, kCacheBadPage);
+              page = -1;
+            }
           }
+        } else if (first >= 0) {  // its rows become zeros
+          rows = min(max(count - j * kCacheBlock, 0), kCacheBlock);
+          row = first + j * kCacheBlock;
+          if (rows > 0) report(p.status, good ? kCacheBadLength : kCacheBadSlot);
         }
       }
-      info[r] = ti;
+      at_rows = rows, at_written = written, at_row = row, at_pos = pos, at_page = page;
     }
+  } else if (threadIdx.x < 32 + 2 * kHeads) {
+    (&tops[0][0])[threadIdx.x - 32] = 0;
+    (&poisoned[0][0])[threadIdx.x - 32] = 0;
+  }
+  if (blockIdx.x == gridDim.x - 1) {  // rows that belong to no sequence
+    const int from = p.n > 0 ? min(max(p.cu[p.n], 0), p.tokens) : 0;
+    uint4* o = reinterpret_cast<uint4*>(p.q_out);
+    const int64_t per = (int64_t)p.H * kCacheDim / 8;
+    if (blockIdx.y == 0)
+      for (int64_t x = from * per + threadIdx.x; x < p.tokens * per; x += kAppendThreads) o[x] = make_uint4(0, 0, 0, 0);
   }
   __syncthreads();
+  const int rows = at_rows, written = at_written, pos0 = at_pos, page = at_page;
+  if (rows == 0) return;
+  const int h0 = blockIdx.y * kHeads, heads = min(kHeads, p.KV - h0), group = p.H / p.KV;
+  const T* k = reinterpret_cast<const T*>(p.k) + at_row * p.k_tok + h0 * p.k_head + d;
+  const T* v = reinterpret_cast<const T*>(p.v) + at_row * p.v_tok + h0 * p.v_head + d;
+  const T* q = reinterpret_cast<const T*>(p.q) + at_row * p.q_tok + (int64_t)h0 * group * p.q_head + d;
+  T* out = reinterpret_cast<T*>(p.q_out) + ((int64_t)at_row * p.H + (int64_t)h0 * group) * kCacheDim + d;
+  const float* cos = p.cos + (int64_t)pos0 * kCacheDim + d;
+  const float* sin = p.sin + (int64_t)pos0 * kCacheDim + d;
+  const int writes = page >= 0 ? written : 0;
 
-  const int kvh = blockIdx.y, group = p.H / p.KV;
-  const int half = lane >> 4, d = (lane & 15) * 4;
-  // ---- keys and values: item 2r is the keys of the block that row r leads, 2r + 1 its values
-  for (int item = warp; item < 2 * here; item += kAppendThreads / 32) {
-    const TokenInfo ti = info[item >> 1];
-    if (ti.count == 0 || ti.page < 0) continue;
-    const bool is_v = item & 1;
-    const int t = t0 + (item >> 1);
-    const T* src = is_v ? p.v + kvh * p.v_head : p.k + kvh * p.k_head;
-    const int64_t tok = is_v ? p.v_tok : p.k_tok;
-    float4 lo[8], hi[8];
-    float amax = 0.f;
-    bool bad = false;
+  // ---- keys and values: up to kHeads items a team, held until their scale is known
+  float4 klo[kHeads], khi[kHeads];
+  uint2 vr[kHeads][2];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 2 * i + half;
-      lo[i] = hi[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < ti.count) {
-        lo[i] = load4(src + (t + r) * tok + d);
-        hi[i] = load4(src + (t + r) * tok + 64 + d);
-      }
+  for (int i = 0; i < kHeads; ++i) {
+    const int item = team + i * kTeams, r = item % rows, h = item / rows;
+    klo[i] = khi[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    vr[i][0] = vr[i][1] = make_uint2(0, 0);
+    if (h < heads && r < writes) {
+      const T* ks = k + r * p.k_tok + h * p.k_head;
+      const T* vs = v + r * p.v_tok + h * p.v_head;
+      klo[i] = widen<T>(raw4(ks)), khi[i] = widen<T>(raw4(ks + 64));
+      vr[i][0] = raw4(vs), vr[i][1] = raw4(vs + 64);
     }
-    if (!is_v) {
+  }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 2 * i + half;
-        if (r < ti.count) {
-          const int64_t row = (int64_t)(ti.pos + r) * kCacheDim;
-          rotate(lo[i], hi[i], p.cos + row, p.sin + row, d);
-        }
-      }
+  for (int i = 0; i < kHeads; ++i) {
+    const int item = team + i * kTeams, r = item % rows, h = item / rows;
+    if (i * kTeams >= rows * heads) break;  // the same for the whole block: the shuffles below are the warp's
+    const bool held = h < heads && r < writes;
+    if (held) {
+      const float* c = cos + r * kCacheDim;
+      const float* s = sin + r * kCacheDim;
+      rotate(klo[i], khi[i], *reinterpret_cast<const float4*>(c), *reinterpret_cast<const float4*>(c + 64),
+             *reinterpret_cast<const float4*>(s), *reinterpret_cast<const float4*>(s + 64));
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      take_finite(lo[i], amax, bad);
-      take_finite(hi[i], amax, bad);
-    }
+    for (int which = 0; which < 2; ++which) {
+      float4 lo = which ? widen<T>(vr[i][0]) : klo[i], hi = which ? widen<T>(vr[i][1]) : khi[i];
+      bool bad = false;
+      uint32_t top = take_finite(lo, bad);
+      top = max(top, take_finite(hi, bad));
+      if (which == 0) klo[i] = lo, khi[i] = hi;
+      if (bad && held) poisoned[h][which] = 1;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    bad = __any_sync(0xffffffffu, bad);
+      for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if ((threadIdx.x & 15) == 0 && held) atomicMax(&tops[h][which], top);
+    }
+  }
+  // ---- queries, while the scales of the heads come together
+#pragma unroll 4
+  for (int item = team; item < rows * heads * group; item += kTeams) {
+    const int r = item % rows, h = item / rows;
+    float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+    if (r < written) {
+      const T* src = q + r * p.q_tok + h * p.q_head;
+      const float* c = cos + r * kCacheDim;
+      const float* s = sin + r * kCacheDim;
+      lo = widen<T>(raw4(src)), hi = widen<T>(raw4(src + 64));
+      rotate(lo, hi, *reinterpret_cast<const float4*>(c), *reinterpret_cast<const float4*>(c + 64),
+             *reinterpret_cast<const float4*>(s), *reinterpret_cast<const float4*>(s + 64));
+    }
+    T* dst = out + ((int64_t)r * p.H + h) * kCacheDim;
+    store4(dst, lo);
+    store4(dst + 64, hi);
+  }
+  if (writes == 0) return;
+  __syncthreads();
 
-    const int in_page = ti.pos % p.page, off = ti.pos % kCacheBlock;
-    const int64_t head = ((int64_t)ti.page * 2 + (is_v ? 1 : 0)) * p.KV + kvh;
-    float* scale = p.scales + head * (p.page / kCacheBlock) + in_page / kCacheBlock;
-    uint8_t* base = p.pages + (head * p.page + (in_page - off)) * kCacheDim;  // the block's first token
-    int e = scale_exponent(amax);
+  const int in_page = pos0 % p.page, off = pos0 % kCacheBlock;
+  auto head_of = [&](int h, int which) { return ((int64_t)page * 2 + which) * p.KV + h0 + h; };
+  // ---- a team settles a scale, and rounds the block's older tokens again if it grew
+  if (team < 2 * heads) {
+    const int h = team >> 1, which = team & 1;
+    bool bad = poisoned[h][which] != 0;
+    int e = scale_exponent(__uint_as_float(tops[h][which]));
+    float* scale = p.scales + head_of(h, which) * (p.page / kCacheBlock) + in_page / kCacheBlock;
     if (off > 0) {
       const float was = *scale;
       if (!(fabsf(was) <= 3.402823466e38f)) {
         bad = true;
       } else {
         const int e_was = (__float_as_int(was) >> 23) - 127;
-        if (e > e_was) {  // older tokens are rounded again
+        if (e > e_was) {
           const float f = e - e_was < 127 ? two_to(e_was - e) : 0.f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int r = 2 * i + half;
-            if (r < off) {
-              uint2* b = reinterpret_cast<uint2*>(base + r * kCacheDim) + (lane & 15);
-              const uint2 w = *b;
-              *b = make_uint2(to_e4m3(times(from_e4m3(w.x), f)), to_e4m3(times(from_e4m3(w.y), f)));
-            }
+          uint2* b = reinterpret_cast<uint2*>(p.pages + (head_of(h, which) * p.page + in_page - off) * kCacheDim) + (threadIdx.x & 15);
+#pragma unroll 4
+          for (int r = 0; r < off; ++r) {
+            const uint2 w = b[r * (kCacheDim / 8)];
+            b[r * (kCacheDim / 8)] = make_uint2(to_e4m3(times(from_e4m3(w.x), f)), to_e4m3(times(from_e4m3(w.y), f)));
           }
         }
         e = max(e, e_was);
       }
     }
-    const float inv = two_to(-e);  // -120 <= -e <= 32
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int r = 2 * i + half;
-      if (r < ti.count) {
-        uint8_t* b = base + (off + r) * kCacheDim + d;
-        *reinterpret_cast<uint32_t*>(b) = to_e4m3(times(lo[i], inv));
-        *reinterpret_cast<uint32_t*>(b + 64) = to_e4m3(times(hi[i], inv));
-      }
+    __syncwarp(0xffffu << (threadIdx.x & 16));  // the team has read the old scale
+    if ((threadIdx.x & 15) == 0) {
+      exponents[h][which] = e;
+      *scale = bad ? __int_as_float(0x7fc00000) : two_to(e);
     }
-    __syncwarp();  // every lane has read the old scale
-    if (lane == 0) *scale = bad ? __int_as_float(0x7fc00000) : two_to(e);
   }
-  // ---- queries: two rows (token, head of the group) a warp
-  for (int item = warp * 2 + half; item < here * group; item += kAppendThreads / 16) {
-    const int r = item / group, h = kvh * group + item % group;
-    const TokenInfo ti = info[r];
-    float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
-    if (ti.pos >= 0) {
-      const T* src = p.q + (t0 + r) * p.q_tok + h * p.q_head;
-      lo = load4(src + d);
-      hi = load4(src + 64 + d);
-      const int64_t row = (int64_t)ti.pos * kCacheDim;
-      rotate(lo, hi, p.cos + row, p.sin + row, d);
+  __syncthreads();
+  // ---- bytes
+#pragma unroll
+  for (int i = 0; i < kHeads; ++i) {
+    const int item = team + i * kTeams, r = item % rows, h = item / rows;
+    if (h >= heads || r >= writes) continue;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      float4 lo = which ? widen<T>(vr[i][0]) : klo[i], hi = which ? widen<T>(vr[i][1]) : khi[i];
+      bool bad;
+      if (which) take_finite(lo, bad), take_finite(hi, bad);
+      const float inv = two_to(-exponents[h][which]);  // -120 <= -e <= 32
+      uint8_t* b = p.pages + (head_of(h, which) * p.page + in_page + r) * kCacheDim + d;
+      *reinterpret_cast<uint32_t*>(b) = to_e4m3(times(lo, inv));
+      *reinterpret_cast<uint32_t*>(b + 64) = to_e4m3(times(hi, inv));
     }
-    T* dst = p.q_out + ((int64_t)(t0 + r) * p.H + h) * kCacheDim;
-    store4(dst + d, lo);
-    store4(dst + 64 + d, hi);
   }
 }
 
 template <typename T>
-void launch_append(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cos,
-                   const at::Tensor& sin, const at::Tensor& pages, const at::Tensor& scales, const at::Tensor& table,
-                   const at::Tensor& lens, const at::Tensor& seqs, const at::Tensor& cu, at::Tensor& out) {
-  AppendParams<T> p{};
-  p.q = reinterpret_cast<const T*>(q.data_ptr());
-  p.k = reinterpret_cast<const T*>(k.data_ptr());
-  p.v = reinterpret_cast<const T*>(v.data_ptr());
-  p.q_tok = q.stride(0), p.q_head = q.stride(1);
-  p.k_tok = k.stride(0), p.k_head = k.stride(1);
-  p.v_tok = v.stride(0), p.v_head = v.stride(1);
-  p.q_out = reinterpret_cast<T*>(out.data_ptr());
-  p.cos = cos.data_ptr<float>(), p.sin = sin.data_ptr<float>();
-  p.positions = cos.size(0);
-  p.pages = reinterpret_cast<uint8_t*>(pages.data_ptr());
-  p.scales = scales.data_ptr<float>();
-  p.npages = pages.size(0);
-  p.table = table.data_ptr<int>(), p.lens = lens.data_ptr<int>();
-  p.seqs = seqs.data_ptr<int>(), p.cu = cu.data_ptr<int>();
-  p.slots = (int)table.size(0), p.width = (int)table.size(1), p.n = (int)seqs.size(0);
-  p.tokens = (int)q.size(0), p.H = (int)q.size(1), p.KV = (int)k.size(1), p.page = (int)pages.size(3);
-  // Few tokens: more and smaller blocks, so that every block of 16 tokens has a warp at once.
-  p.chunk = p.tokens >= 2048 ? kMaxChunk : 4;
-  p.status = cache_status_word(q.device());
-  const dim3 grid((unsigned)((p.tokens + p.chunk - 1) / p.chunk), (unsigned)p.KV);
-  cache_append_kernel<T><<<grid, kAppendThreads, 0, at::cuda::getCurrentCUDAStream()>>>(p);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+cudaError_t launch_append(const AppendParams& p, cudaStream_t stream) {
+  const dim3 grid(p.tokens / kCacheBlock + 3 * p.n + 1, (p.KV + kHeads - 1) / kHeads);
+  cache_append_kernel<T><<<grid, kAppendThreads, 0, stream>>>(p);
+  return cudaGetLastError();
 }
 
 // ---------------------------------------------------------------------------------- pages
 constexpr int kBook = 1024;        // threads of the bookkeeping block
-constexpr int kMaxBatch = 4096;    // sequences of one call
+constexpr int kMaxBatch = kBookBatch;
 constexpr int kPer = 8;            // pages that one thread looks at in a step
 
 // Exclusive sum of x over the block (kBook threads); `total` gets the sum.
@@ -436,90 +439,100 @@ __global__ void cache_free_kernel(int* table, int slots, int width, int* lens, i
   if (threadIdx.x == 0) lens[slot] = 0;
 }
 
-// Slot dst[i] gives up its pages and takes those of src[i] that are full; part[i] = the page that
-// has to be copied, or -1.
-__global__ void cache_share_kernel(int* table, int slots, int width, int* lens, int* refs, int npages, const int* src,
-                                   const int* dst, int page, int* part, int* status) {
-  const int i = blockIdx.x, a = src[i], b = dst[i];
-  if (a < 0 || a >= slots || b < 0 || b >= slots || a == b) {
-    if (threadIdx.x == 0) {
-      report(status, kCacheBadSlot);
-      part[i] = -2;
-    }
-    return;
-  }
-  const int len = lens[a], whole = min(len / page, width);
-  for (int j = threadIdx.x; j < width; j += blockDim.x) {
-    const int old = atomicExch(table + (int64_t)b * width + j, -1);
-    if (old >= npages) report(status, kCacheBadPage);
-    else if (old >= 0) atomicSub(refs + old, 1);
-    if (j < whole) {
-      const int shared = table[(int64_t)a * width + j];
-      if (shared < 0 || shared >= npages) {
-        report(status, kCacheBadPage);
-      } else {
-        table[(int64_t)b * width + j] = shared;
-        atomicAdd(refs + shared, 1);
-      }
-    }
-  }
-  if (threadIdx.x == 0) {
-    lens[b] = len;
-    int last = -1;
-    if (len % page != 0) {
-      last = whole < width ? table[(int64_t)a * width + whole] : -1;
-      if (last < 0 || last >= npages) {
-        report(status, kCacheBadPage);
-        last = -1;
-      }
-    }
-    part[i] = last;
-  }
-}
-
-// Fresh pages for the partly filled ones: copy lists from[i] -> to[i] (-1: nothing), lowest free
-// page first in the order of the batch.  Where pages lack, every destination is left empty.
-__global__ void __launch_bounds__(kBook) cache_fork_kernel(int* table, int width, int* lens, int* refs, int npages,
-                                                           const int* dst, int n, int page, int* from, int* to,
-                                                           int* found, int* missing) {
+// Slot dst[i] gives up its pages, takes those of src[i] that are full, and a free one for a last page
+// that is not: the copy list from[i] -> to[i] (-1: nothing to copy, -2: a bad pair), lowest free page
+// first in the order of the batch.  Where pages lack, every destination is left empty.
+// One block: the entries of all pairs' rows are gone through by its threads, four ahead.
+__global__ void __launch_bounds__(kBook) cache_fork_kernel(const Book b, const int* src, const int* dst, int n, int* from,
+                                                           int* to, int* found, int* missing) {
   __shared__ int need[kMaxBatch];
   __shared__ int warp_sums[32];
-  for (int i = threadIdx.x; i < n; i += kBook) need[i] = from[i] >= 0;
+  const int64_t entries = (int64_t)n * b.width;
+  auto good = [&](int s, int d) { return s >= 0 && s < b.slots && d >= 0 && d < b.slots && s != d; };
+  for (int64_t base = threadIdx.x; base < entries; base += 4 * kBook) {
+    int old[4], shared[4];
+    int* entry[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int64_t k = base + x * kBook;
+      old[x] = shared[x] = -1;
+      entry[x] = nullptr;
+      if (k >= entries) continue;
+      const int i = (int)(k / b.width), j = (int)(k % b.width), s = src[i], d = dst[i];
+      if (!good(s, d)) continue;
+      entry[x] = b.table + (int64_t)d * b.width + j;
+      old[x] = *entry[x];
+      if (j < b.lens[s] / b.page) {
+        shared[x] = b.table[(int64_t)s * b.width + j];
+        if (shared[x] < 0 || shared[x] >= b.npages) {
+          report(b.status, kCacheBadPage);
+          shared[x] = -1;
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if (entry[x] == nullptr) continue;
+      *entry[x] = shared[x];
+      if (shared[x] >= 0) atomicAdd(b.refs + shared[x], 1);
+      if (old[x] >= b.npages) report(b.status, kCacheBadPage);
+      else if (old[x] >= 0) atomicSub(b.refs + old[x], 1);
+    }
+  }
+  for (int i = threadIdx.x; i < n; i += kBook) {
+    const int s = src[i], d = dst[i];
+    int last = -1;
+    if (!good(s, d)) {
+      report(b.status, kCacheBadSlot);
+      last = -2;
+    } else {
+      const int len = b.lens[s], whole = len / b.page;
+      if (len % b.page != 0) {
+        last = whole < b.width ? b.table[(int64_t)s * b.width + whole] : -1;
+        if (last < 0 || last >= b.npages) {
+          report(b.status, kCacheBadPage);
+          last = -1;
+        }
+      }
+    }
+    from[i] = last;
+    need[i] = last >= 0;
+  }
   __syncthreads();
+  for (int i = threadIdx.x; i < n; i += kBook)  // after every source length has been read
+    if (from[i] != -2) b.lens[dst[i]] = b.lens[src[i]];
   const int total = scan_needs(need, n, warp_sums);
-  const int have = find_free(refs, npages, min(total, npages), found, warp_sums);
+  const int have = find_free(b.refs, b.npages, min(total, b.npages), found, warp_sums);
   const bool ok = have >= total;
   for (int i = threadIdx.x; i < n; i += kBook) {
-    const bool mine = from[i] >= 0;
     to[i] = -1;
-    if (ok && mine) {
-      const int fresh = found[need[i]], b = dst[i];
+    if (ok && from[i] >= 0) {
+      const int fresh = found[need[i]], d = dst[i];
       to[i] = fresh;
-      table[(int64_t)b * width + lens[b] / page] = fresh;
-      refs[fresh] = 1;
+      b.table[(int64_t)d * b.width + b.lens[d] / b.page] = fresh;
+      b.refs[fresh] = 1;
     }
   }
   if (!ok) {
     __syncthreads();
-    for (int64_t k = threadIdx.x; k < (int64_t)n * width; k += kBook) {
-      const int i = (int)(k / width);
+    for (int64_t k = threadIdx.x; k < entries; k += kBook) {
+      const int i = (int)(k / b.width);
       if (from[i] == -2) continue;
-      int* entry = table + (int64_t)dst[i] * width + k % width;
-      const int old = *entry;
-      if (old >= 0 && old < npages) atomicSub(refs + old, 1);
+      int* entry = b.table + (int64_t)dst[i] * b.width + k % b.width;
+      if (*entry >= 0) atomicSub(b.refs + *entry, 1);
       *entry = -1;
     }
-    __syncthreads();
     for (int i = threadIdx.x; i < n; i += kBook)
-      if (from[i] != -2) lens[dst[i]] = 0;
+      if (from[i] != -2) b.lens[dst[i]] = 0;
   }
   if (threadIdx.x == 0) *missing = ok ? 0 : total - have;
 }
 
 // Where live pages go: those below `live` (their number) stay, the j-th live page from there on
-// goes to the j-th free one below.  to[p] = -1 for a free page.
-__global__ void __launch_bounds__(kBook) cache_plan_kernel(const int* refs, int npages, int room, int* holes, int* to,
-                                                           int* missing) {
+// goes to the j-th free one below.  to[p] = -1 for a free page.  The counts go along: out_refs may
+// be refs itself (a move in place), so they are kept in between.
+__global__ void __launch_bounds__(kBook) cache_plan_kernel(const int* refs, int npages, int* out_refs, int room, int* holes,
+                                                           int* to, int* kept, int* missing) {
   __shared__ int warp_sums[32];
   int live = 0;
   for (int base = 0; base < npages; base += kBook * kPer) {
@@ -527,14 +540,18 @@ __global__ void __launch_bounds__(kBook) cache_plan_kernel(const int* refs, int 
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int p = base + (int)threadIdx.x * kPer + i;
-      c += p < npages && refs[p] != 0;
+      if (p < npages) {
+        const int count = refs[p];
+        kept[p] = count;
+        c += count != 0;
+      }
     }
     int total;
     block_scan(c, warp_sums, total);
     live += total;
   }
   if (threadIdx.x == 0) *missing = max(live - room, 0);
-  find_free(refs, live, live, holes, warp_sums);
+  find_free(refs, min(live, npages), live, holes, warp_sums);
   int moved = 0;
   for (int base = 0; base < npages; base += kBook * kPer) {
     const int first = base + (int)threadIdx.x * kPer;
@@ -542,7 +559,7 @@ __global__ void __launch_bounds__(kBook) cache_plan_kernel(const int* refs, int 
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int p = first + i;
-      if (p < npages && refs[p] != 0) {
+      if (p < npages && kept[p] != 0) {
         mask |= 1 << i;
         if (p >= live) above |= 1 << i;
       }
@@ -556,28 +573,17 @@ __global__ void __launch_bounds__(kBook) cache_plan_kernel(const int* refs, int 
     }
     moved += total;
   }
+  if (live > room) return;
+  __syncthreads();
+  for (int p = threadIdx.x; p < room; p += kBook) out_refs[p] = 0;
+  __syncthreads();
+  for (int p = threadIdx.x; p < npages; p += kBook)
+    if (to[p] >= 0) out_refs[to[p]] = kept[p];
 }
 
+// A block takes a whole page of a layer at a time, 32 KB in flight.
 constexpr int kCopyThreads = 256;
-constexpr int kCopyBytes = kCopyThreads * 16 * 4;  // one block's share of a page in a step
-
-// Copies page from[i] of every layer to page to[i] (i itself where `from` is null; nothing where
-// either is negative or both are the same page of one pool), bytes and scales.
-struct CopyParams {
-  const uint8_t* pages;
-  const float* scales;
-  uint8_t* out_pages;
-  float* out_scales;
-  int64_t npages, out_npages;
-  int64_t page_bytes;
-  int scale_floats, layers, n;
-  const int *from, *to, *missing;
-  int* status;
-  // compaction: the table and the counts of the new pool
-  const int *table, *refs;
-  int *out_table, *out_refs;
-  int64_t entries;
-};
+constexpr int kCopyAhead = 8;
 
 __device__ __forceinline__ bool copy_item(const CopyParams& p, int i, int& a, int& b) {
   a = p.from != nullptr ? p.from[i] : i;
@@ -590,33 +596,31 @@ __device__ __forceinline__ bool copy_item(const CopyParams& p, int i, int& a, in
   return !(a == b && p.pages == p.out_pages);
 }
 
+// blockIdx.y: layer; blockIdx.x: a share of the list.
 __global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const CopyParams p) {
   if (p.missing != nullptr && *p.missing != 0) return;
-  const int64_t parts = (p.page_bytes + kCopyBytes - 1) / kCopyBytes;
-  const int64_t total = parts * p.n * p.layers;
-  for (int64_t w = blockIdx.x; w < total; w += gridDim.x) {
-    const int64_t part = w % parts, rest = w / parts;
-    const int i = (int)(rest % p.n);
-    const int64_t layer = rest / p.n;
+  const int end = (int)(p.page_bytes / 16);
+  for (int i = blockIdx.x; i < p.n; i += gridDim.x) {
     int a, b;
     if (!copy_item(p, i, a, b)) continue;
-    const int64_t in = layer * p.npages + a, out = layer * p.out_npages + b;
+    const int64_t in = blockIdx.y * p.npages + a, out = blockIdx.y * p.out_npages + b;
     const uint4* s = reinterpret_cast<const uint4*>(p.pages + in * p.page_bytes);
     uint4* o = reinterpret_cast<uint4*>(p.out_pages + out * p.page_bytes);
-    const int64_t end = p.page_bytes / 16, first = part * (kCopyBytes / 16) + threadIdx.x;
-    uint4 v[4];
+    for (int first = threadIdx.x; first < end; first += kCopyThreads * kCopyAhead) {
+      uint4 v[kCopyAhead];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (first + u * kCopyThreads < end) v[u] = s[first + u * kCopyThreads];
+      for (int u = 0; u < kCopyAhead; ++u)
+        if (first + u * kCopyThreads < end) v[u] = __ldcs(s + first + u * kCopyThreads);
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (first + u * kCopyThreads < end) o[first + u * kCopyThreads] = v[u];
-    if (part == 0)
-      for (int f = threadIdx.x; f < p.scale_floats; f += kCopyThreads)
-        p.out_scales[out * p.scale_floats + f] = p.scales[in * p.scale_floats + f];
+      for (int u = 0; u < kCopyAhead; ++u)
+        if (first + u * kCopyThreads < end) __stcs(o + first + u * kCopyThreads, v[u]);
+    }
+    for (int f = threadIdx.x; f < p.scale_floats; f += kCopyThreads)
+      p.out_scales[out * p.scale_floats + f] = p.scales[in * p.scale_floats + f];
   }
   if (p.out_table != nullptr) {
-    for (int64_t k = blockIdx.x * (int64_t)kCopyThreads + threadIdx.x; k < p.entries; k += (int64_t)gridDim.x * kCopyThreads) {
+    const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, blocks = (int64_t)gridDim.x * gridDim.y;
+    for (int64_t k = block * kCopyThreads + threadIdx.x; k < p.entries; k += blocks * kCopyThreads) {
       const int page = p.table[k];
       int to = -1;
       if (page >= p.npages) report(p.status, kCacheBadPage);
@@ -626,244 +630,46 @@ __global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const CopyPara
   }
 }
 
-// Counts of a compacted pool: page to[p] of the new pool has the count of page p, the rest are free.
-__global__ void cache_counts_kernel(const int* refs, const int* to, int npages, int* out_refs, const int* missing) {
-  if (*missing != 0) return;
-  for (int p = blockIdx.x * blockDim.x + threadIdx.x; p < npages; p += gridDim.x * blockDim.x)
-    if (to[p] >= 0) out_refs[to[p]] = refs[p];
-}
-__global__ void cache_zero_counts_kernel(int* out_refs, int n, const int* missing) {
-  if (*missing != 0) return;
-  for (int p = blockIdx.x * blockDim.x + threadIdx.x; p < n; p += gridDim.x * blockDim.x) out_refs[p] = 0;
-}
-
-void launch_copy(CopyParams p, const at::Tensor& pages) {
-  p.page_bytes = pages.size(2) * pages.size(3) * pages.size(4) * pages.size(5);
-  p.scale_floats = (int)(p.page_bytes / kCacheDim / kCacheBlock);
-  p.layers = (int)pages.size(0);
-  p.npages = pages.size(1);
-  const int64_t parts = (p.page_bytes + kCopyBytes - 1) / kCopyBytes * p.n * p.layers;
-  const int64_t work = std::max<int64_t>(parts, p.out_table != nullptr ? (p.entries + kCopyThreads - 1) / kCopyThreads : 0);
-  if (work == 0) return;
-  cache_copy_kernel<<<(unsigned)std::min<int64_t>(work, 148 * 8), kCopyThreads, 0, at::cuda::getCurrentCUDAStream()>>>(p);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-}
-
-void check_book(const at::Tensor& table, const at::Tensor& lens, const at::Tensor& refs) {
-  CACHE_CHECK(table.is_cuda(), "page_table must be a CUDA tensor");
-  check_int32(table, "page_table", 2, table.device());
-  check_int32(lens, "seq_lens", 1, table.device());
-  check_int32(refs, "ref_counts", 1, table.device());
-  CACHE_CHECK(lens.size(0) == table.size(0), "seq_lens needs one length for each row of page_table");
-  CACHE_CHECK(refs.size(0) < (int64_t(1) << 30), "the pool has too many pages");
-}
-
-void check_page_size(int64_t page) {
-  CACHE_CHECK(page >= 16 && page <= 256 && (page & (page - 1)) == 0, "page_size must be 16, 32, 64, 128 or 256, not ",
-              page);
-}
-
 }  // namespace
 
 namespace mimir {
-int* cache_status_word(const at::Device& dev) {
-  static int* words[64] = {nullptr};
-  const int i = dev.index();
-  if (words[i] == nullptr) {
-    c10::cuda::CUDAGuard guard(dev);
-    void* ptr = nullptr;
-    C10_CUDA_CHECK(cudaGetSymbolAddress(&ptr, g_cache_status));
-    words[i] = reinterpret_cast<int*>(ptr);
-  }
-  return words[i];
+
+cudaError_t cache_status_address(void** word) { return cudaGetSymbolAddress(word, g_cache_status); }
+
+cudaError_t launch_cache_append(const AppendParams& p, bool bf16, cudaStream_t stream) {
+  return bf16 ? launch_append<__nv_bfloat16>(p, stream) : launch_append<__half>(p, stream);
 }
+
+cudaError_t launch_cache_reserve(const Book& b, const int* seqs, const int* counts, int n, int* found, int* missing,
+                                 cudaStream_t stream) {
+  cache_reserve_kernel<<<1, kBook, 0, stream>>>(b.table, b.slots, b.width, b.lens, b.refs, b.npages, seqs, counts, n, b.page,
+                                                found, missing);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_cache_free(const Book& b, const int* seqs, int n, cudaStream_t stream) {
+  cache_free_kernel<<<n, 256, 0, stream>>>(b.table, b.slots, b.width, b.lens, b.refs, b.npages, seqs, b.status);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_cache_fork(const Book& b, const int* src, const int* dst, int n, int* from, int* to, int* found,
+                              int* missing, cudaStream_t stream) {
+  cache_fork_kernel<<<1, kBook, 0, stream>>>(b, src, dst, n, from, to, found, missing);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_cache_plan(const int* refs, int npages, int* out_refs, int room, int* holes, int* to, int* kept,
+                              int* missing, cudaStream_t stream) {
+  cache_plan_kernel<<<1, kBook, 0, stream>>>(refs, npages, out_refs, room, holes, to, kept, missing);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_cache_copy(const CopyParams& p, cudaStream_t stream) {
+  if (p.layers == 0 || (p.n == 0 && p.entries == 0)) return cudaSuccess;
+  const int y = std::min(p.layers, 65535);
+  const int x = std::min(std::max(p.n, 1), std::max(1, 148 * 8 / y));
+  cache_copy_kernel<<<dim3(x, y), kCopyThreads, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
 }  // namespace mimir
-
-// The first status code of a cache kernel since the last read (0: none).
-int64_t cache_status(int64_t device) {
-  c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
-  int* word = cache_status_word(at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
-  int host = 0;
-  C10_CUDA_CHECK(cudaStreamSynchronize(at::cuda::getCurrentCUDAStream()));  // this stream's kernels have reported
-  C10_CUDA_CHECK(cudaMemcpy(&host, word, sizeof(int), cudaMemcpyDeviceToHost));
-  if (host) C10_CUDA_CHECK(cudaMemset(word, 0, sizeof(int)));
-  return host;
-}
-
-at::Tensor cache_append(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cos, at::Tensor sin, at::Tensor pages,
-                        at::Tensor scales, at::Tensor table, at::Tensor lens, at::Tensor seqs, at::Tensor cu_new) {
-  check_pool(pages, scales, 0);
-  const at::Device dev = pages.device();
-  check_rows(q, "q", dev);
-  check_rows(k, "k", dev);
-  check_rows(v, "v", dev);
-  check_batch(table, lens, seqs, cu_new, dev);
-  CACHE_CHECK(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(), "q, k and v must have one type");
-  CACHE_CHECK(k.size(1) == pages.size(2) && v.size(1) == pages.size(2), "k and v must have the pages' ", pages.size(2),
-              " heads");
-  CACHE_CHECK(k.size(0) == q.size(0) && v.size(0) == q.size(0), "q, k and v must have as many tokens");
-  CACHE_CHECK(q.size(1) >= 1 && q.size(1) % k.size(1) == 0, "query heads ", q.size(1),
-              " must be divisible by key/value heads ", k.size(1));
-  for (const at::Tensor* t : {&cos, &sin})
-    CACHE_CHECK(t->device() == dev && t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(1) == kCacheDim &&
-                    t->is_contiguous() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
-                "cos and sin must be contiguous float32 tables [positions, 128]");
-  CACHE_CHECK(cos.size(0) == sin.size(0), "cos and sin must have as many positions");
-  CACHE_CHECK(q.size(0) < (int64_t(1) << 31) - 64 && k.size(1) < 65536, "too many tokens or heads");
-  c10::cuda::CUDAGuard guard(dev);
-  at::Tensor out = at::empty({q.size(0), q.size(1), kCacheDim}, q.options());
-  if (q.size(0) == 0) return out;
-  if (q.scalar_type() == at::kBFloat16)
-    launch_append<__nv_bfloat16>(q, k, v, cos, sin, pages, scales, table, lens, seqs, cu_new, out);
-  else
-    launch_append<__half>(q, k, v, cos, sin, pages, scales, table, lens, seqs, cu_new, out);
-  return out;
-}
-
-at::Tensor cache_reserve(at::Tensor table, at::Tensor lens, at::Tensor refs, at::Tensor seqs, at::Tensor counts,
-                         int64_t page) {
-  check_book(table, lens, refs);
-  check_int32(seqs, "seqs", 1, table.device());
-  check_int32(counts, "counts", 1, table.device());
-  check_page_size(page);
-  const int64_t n = seqs.size(0);
-  CACHE_CHECK(counts.size(0) == n, "counts needs one entry for each of seqs");
-  CACHE_CHECK(n <= kMaxBatch, "at most ", kMaxBatch, " sequences a call");
-  c10::cuda::CUDAGuard guard(table.device());
-  // [missing | free pages found]
-  const int64_t most = std::min<int64_t>(n * table.size(1), refs.size(0));
-  at::Tensor work = at::empty({1 + std::max<int64_t>(most, 1)}, refs.options());
-  int* w = work.data_ptr<int>();
-  cache_reserve_kernel<<<1, kBook, 0, at::cuda::getCurrentCUDAStream()>>>(
-      table.data_ptr<int>(), (int)table.size(0), (int)table.size(1), lens.data_ptr<int>(), refs.data_ptr<int>(),
-      (int)refs.size(0), seqs.data_ptr<int>(), counts.data_ptr<int>(), (int)n, (int)page, w + 1, w);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return work.narrow(0, 0, 1);
-}
-
-void cache_free(at::Tensor table, at::Tensor lens, at::Tensor refs, at::Tensor seqs) {
-  check_book(table, lens, refs);
-  check_int32(seqs, "seqs", 1, table.device());
-  if (seqs.size(0) == 0) return;
-  c10::cuda::CUDAGuard guard(table.device());
-  cache_free_kernel<<<(unsigned)seqs.size(0), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-      table.data_ptr<int>(), (int)table.size(0), (int)table.size(1), lens.data_ptr<int>(), refs.data_ptr<int>(),
-      (int)refs.size(0), seqs.data_ptr<int>(), cache_status_word(table.device()));
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-}
-
-at::Tensor cache_fork(at::Tensor pages, at::Tensor scales, at::Tensor table, at::Tensor lens, at::Tensor refs,
-                      at::Tensor src, at::Tensor dst) {
-  check_pool(pages, scales, 1);
-  check_book(table, lens, refs);
-  CACHE_CHECK(table.device() == pages.device(), "page_table and pages must be on one device");
-  check_int32(src, "src", 1, table.device());
-  check_int32(dst, "dst", 1, table.device());
-  CACHE_CHECK(refs.size(0) == pages.size(1), "ref_counts needs one count for each page");
-  const int64_t n = src.size(0);
-  CACHE_CHECK(dst.size(0) == n, "src and dst must have as many slots");
-  CACHE_CHECK(n <= kMaxBatch, "at most ", kMaxBatch, " sequences a call");
-  c10::cuda::CUDAGuard guard(table.device());
-  at::Tensor work = at::empty({1 + 3 * std::max<int64_t>(n, 1)}, refs.options());  // missing | from | to | found
-  int* w = work.data_ptr<int>();
-  const int page = (int)pages.size(4), width = (int)table.size(1), np = (int)refs.size(0);
-  auto st = at::cuda::getCurrentCUDAStream();
-  if (n > 0) {
-    cache_share_kernel<<<(unsigned)n, 256, 0, st>>>(table.data_ptr<int>(), (int)table.size(0), width, lens.data_ptr<int>(),
-                                                    refs.data_ptr<int>(), np, src.data_ptr<int>(), dst.data_ptr<int>(),
-                                                    page, w + 1, cache_status_word(table.device()));
-    C10_CUDA_KERNEL_LAUNCH_CHECK();
-  }
-  cache_fork_kernel<<<1, kBook, 0, st>>>(table.data_ptr<int>(), width, lens.data_ptr<int>(), refs.data_ptr<int>(), np,
-                                         dst.data_ptr<int>(), (int)n, page, w + 1, w + 1 + n, w + 1 + 2 * n, w);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  if (n > 0) {
-    CopyParams p{};
-    p.pages = reinterpret_cast<const uint8_t*>(pages.data_ptr());
-    p.out_pages = reinterpret_cast<uint8_t*>(pages.data_ptr());
-    p.scales = scales.data_ptr<float>();
-    p.out_scales = scales.data_ptr<float>();
-    p.out_npages = pages.size(1);
-    p.n = (int)n;
-    p.from = w + 1;
-    p.to = w + 1 + n;
-    p.missing = w;
-    p.status = cache_status_word(table.device());
-    launch_copy(p, pages);
-  }
-  return work.narrow(0, 0, 1);
-}
-
-void cache_copy(at::Tensor pages, at::Tensor scales, at::Tensor src, at::Tensor dst) {
-  check_pool(pages, scales, 1);
-  check_int32(src, "src", 1, pages.device());
-  check_int32(dst, "dst", 1, pages.device());
-  CACHE_CHECK(src.size(0) == dst.size(0), "src and dst must have as many pages");
-  c10::cuda::CUDAGuard guard(pages.device());
-  CopyParams p{};
-  p.pages = reinterpret_cast<const uint8_t*>(pages.data_ptr());
-  p.out_pages = reinterpret_cast<uint8_t*>(pages.data_ptr());
-  p.scales = scales.data_ptr<float>();
-  p.out_scales = scales.data_ptr<float>();
-  p.out_npages = pages.size(1);
-  p.n = (int)src.size(0);
-  p.from = src.data_ptr<int>();
-  p.to = dst.data_ptr<int>();
-  p.status = cache_status_word(pages.device());
-  launch_copy(p, pages);
-}
-
-// out_*: another pool (its table the shape of `table`), or the same tensors for a move in place.
-at::Tensor cache_compact(at::Tensor pages, at::Tensor scales, at::Tensor table, at::Tensor refs, at::Tensor out_pages,
-                         at::Tensor out_scales, at::Tensor out_table, at::Tensor out_refs) {
-  check_pool(pages, scales, 1);
-  check_pool(out_pages, out_scales, 1);
-  const at::Device dev = pages.device();
-  check_int32(table, "page_table", 2, dev);
-  check_int32(refs, "ref_counts", 1, dev);
-  check_int32(out_table, "the new page_table", 2, dev);
-  check_int32(out_refs, "the new ref_counts", 1, dev);
-  CACHE_CHECK(out_pages.device() == dev, "both pools must be on one device");
-  CACHE_CHECK(out_table.sizes() == table.sizes(), "the new page_table must have the shape of the old one");
-  CACHE_CHECK(refs.size(0) == pages.size(1) && out_refs.size(0) == out_pages.size(1),
-              "ref_counts needs one count for each page");
-  for (int64_t i : {0, 2, 3, 4, 5})
-    CACHE_CHECK(pages.size(i) == out_pages.size(i), "the new pool must differ in its number of pages only");
-  const bool in_place = pages.data_ptr() == out_pages.data_ptr();
-  CACHE_CHECK(in_place == (table.data_ptr() == out_table.data_ptr()) && in_place == (refs.data_ptr() == out_refs.data_ptr()) &&
-                  in_place == (scales.data_ptr() == out_scales.data_ptr()) &&
-                  (!in_place || pages.size(1) == out_pages.size(1)),
-              "compact into a pool of its own, or in place throughout");
-  c10::cuda::CUDAGuard guard(dev);
-  const int np = (int)refs.size(0);
-  at::Tensor work = at::empty({1 + 3 * (int64_t)std::max(np, 1)}, refs.options());  // missing | to | holes | old counts
-  int* w = work.data_ptr<int>();
-  auto st = at::cuda::getCurrentCUDAStream();
-  cache_plan_kernel<<<1, kBook, 0, st>>>(refs.data_ptr<int>(), np, (int)out_refs.size(0), w + 1 + np, w + 1, w);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  const int* counts = refs.data_ptr<int>();
-  if (in_place && np > 0) {
-    int* kept = w + 1 + 2 * (int64_t)np;
-    C10_CUDA_CHECK(cudaMemcpyAsync(kept, counts, sizeof(int) * np, cudaMemcpyDeviceToDevice, st));
-    counts = kept;
-  }
-  const int on = (int)out_refs.size(0);
-  if (on > 0) cache_zero_counts_kernel<<<std::min(148, (on + 255) / 256), 256, 0, st>>>(out_refs.data_ptr<int>(), on, w);
-  if (np > 0) cache_counts_kernel<<<std::min(148, (np + 255) / 256), 256, 0, st>>>(counts, w + 1, np, out_refs.data_ptr<int>(), w);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  CopyParams p{};
-  p.pages = reinterpret_cast<const uint8_t*>(pages.data_ptr());
-  p.out_pages = reinterpret_cast<uint8_t*>(out_pages.data_ptr());
-  p.scales = scales.data_ptr<float>();
-  p.out_scales = out_scales.data_ptr<float>();
-  p.out_npages = out_pages.size(1);
-  p.n = np;
-  p.to = w + 1;
-  p.missing = w;
-  p.status = cache_status_word(dev);
-  p.table = table.data_ptr<int>();
-  p.out_table = out_table.data_ptr<int>();
-  p.entries = table.numel();
-  launch_copy(p, pages);
-  return work.narrow(0, 0, 1);
-}

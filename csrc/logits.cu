@@ -6,238 +6,228 @@
 //   x = x + the row's biases for v
 //   v not allowed:                           x = -inf
 //
-// in fp32.  A block owns a slice of one row's vocabulary: it counts the row's tokens that fall into
-// its slice in shared memory (whole numbers, so the order of the atomics does not matter), adds the
-// biases there in their order (one warp; equal ids of one step by their first lane, so that sums do
-// not depend on scheduling), and then reads its logits once and writes them once.  The history is
-// read by every block of a row, from L2 after the first.
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
+// in fp32.  A block owns a slice of one row's vocabulary.  A few blocks an SM wait for memory most of
+// their time, so a block asks for all that it can at once: its logits, the row's first 4096 tokens
+// before it knows how many count, the biases before it knows which are its own.  It counts the row's tokens that fall into its slice in shared memory (whole numbers,
+// so the order of the atomics does not matter); the few biases of the slice lie in a list, equal ids
+// summed in their order, and a token's word says which of them is its own.  The history is read by every block of a row, from L2 after the first, so slices are large.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <torch/extension.h>
+
+#include "serving.h"
+
+using namespace mimir;
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kSlice = 4096;
-constexpr uint32_t kSeen = 0x80000000u;  // the token is in the row's history; the rest counts generated ones
-
-template <typename T>
-struct LogitsParams {
-  const T* logits;
-  int64_t ld;
-  float* out;
-  int rows, vocab;
-  const int *tokens, *token_lens, *prompt_lens;
-  int64_t tokens_ld;
-  int tokens_width;
-  const float *repetition, *presence, *frequency;
-  const int *bias_offsets, *bias_ids;
-  const float* bias_values;
-  int bias_count;
-  const int* allowed;
-  int64_t allowed_ld;
-};
+constexpr int kThreads = 512;
+constexpr int kSlice = 8192;               // 32 KB of counts
+constexpr int kEach = kSlice / kThreads;   // logits of a thread
+constexpr int kAhead = 8;                  // tokens of the history that a thread asks for at once
+// A token's word: it is in the row's history; it has a bias, and which (9 bits); how often it was generated.
+constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u;
+constexpr int kHitShift = 21;
+constexpr uint32_t kMadeMask = (1u << kHitShift) - 1;
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) process_logits_kernel(const LogitsParams<T> p) {
-  __shared__ uint32_t counts[kSlice];
-  __shared__ float bias[kSlice];
+struct Four {  // four logits of one load: their four results are one 16-byte store, a warp's lie together
+  using Raw = uint2;
+};
+template <>
+struct Four<float> {
+  using Raw = uint4;
+};
+
+template <typename T, bool kAligned>
+__global__ void __launch_bounds__(kThreads, 3) process_logits_kernel(const LogitsParams p) {
+  __shared__ __align__(16) uint32_t counts[kSlice];
+  __shared__ __align__(16) int hit_ids[kThreads + 4];
+  __shared__ float hit_values[kThreads];
+  __shared__ int warp_hits[kThreads / 32];
+  using Raw = typename Four<T>::Raw;
   const int row = blockIdx.y, v0 = blockIdx.x * kSlice, here = min(kSlice, p.vocab - v0);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const bool with_tokens = p.tokens != nullptr;
+  const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld + v0;
+  float* y = p.out + (int64_t)row * p.vocab + v0;
+  Raw raw[kEach / 4];
+  T single[kAligned ? 1 : kEach];
+  if (kAligned) {
+#pragma unroll
+    for (int u = 0; u < kEach / 4; ++u)
+      if ((u * kThreads + tid) * 4 < here) raw[u] = __ldcs(reinterpret_cast<const Raw*>(x) + u * kThreads + tid);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kEach; ++u)
+      if (u * kThreads + tid < here) single[u] = x[u * kThreads + tid];
+  }
+  const uint32_t* allowed = p.allowed != nullptr ? reinterpret_cast<const uint32_t*>(p.allowed) + row * p.allowed_ld + (v0 >> 5) : nullptr;
+  uint32_t bits[kAligned ? kEach / 4 : 1];
+  if (kAligned) {
+#pragma unroll
+    for (int u = 0; u < kEach / 4; ++u) {
+      const int i = (u * kThreads + tid) * 4;
+      bits[u] = allowed != nullptr && i < here ? allowed[i >> 5] >> (i & 31) : 0xffffffffu;
+    }
+  }
   int b0 = 0, b1 = 0;
   if (p.bias_offsets != nullptr) {
     b0 = max(p.bias_offsets[row], 0);
     b1 = min(p.bias_offsets[row + 1], p.bias_count);
   }
-  const bool with_bias = b1 > b0;
-  if (with_tokens)
-    for (int i = threadIdx.x; i < kSlice; i += kThreads) counts[i] = 0;
-  if (with_bias)
-    for (int i = threadIdx.x; i < kSlice; i += kThreads) bias[i] = 0.f;
-  __syncthreads();
+  const int* ids = p.tokens + row * p.tokens_ld;
+  int held[kAhead];
+#pragma unroll
+  for (int u = 0; u < kAhead; ++u) held[u] = with_tokens && u * kThreads + tid < p.tokens_width ? ids[u * kThreads + tid] : -1;
+  int n = 0, prompt = 0;
   if (with_tokens) {
-    const int n = min(p.token_lens != nullptr ? p.token_lens[row] : p.tokens_width, p.tokens_width);
-    const int prompt = p.prompt_lens != nullptr ? p.prompt_lens[row] : 0;
-    const int* ids = p.tokens + row * p.tokens_ld;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const int at = ids[i] - v0;
-      if (at < 0 || at >= here) continue;
-      if (i >= prompt) atomicAdd(&counts[at], 1u);
-      atomicOr(&counts[at], kSeen);
-    }
+    n = min(p.token_lens != nullptr ? p.token_lens[row] : p.tokens_width, p.tokens_width);
+    prompt = p.prompt_lens != nullptr ? p.prompt_lens[row] : 0;
   }
-  if (with_bias && threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    for (int base = b0; base < b1; base += 32) {
-      const int i = base + lane;
-      int at = -1;
-      float value = 0.f;
-      if (i < b1) {
-        at = p.bias_ids[i] - v0;
-        if (at < 0 || at >= here) at = -1;
-        else value = p.bias_values[i];
-      }
-      if (__any_sync(0xffffffffu, at >= 0)) {
-        const uint32_t same = __match_any_sync(0xffffffffu, at);
-        const bool first = (__ffs(same) - 1) == lane;
-        // the sum of equal ids, lowest lane first
-        float sum = first && at >= 0 ? bias[at] : 0.f;
-        for (int l = 0; l < 32; ++l) {
-          const float x = __shfl_sync(0xffffffffu, value, l);
-          if (same >> l & 1) sum += x;
-        }
-        if (first && at >= 0) bias[at] = sum;
-        __syncwarp();
-      }
-    }
-  }
-  __syncthreads();
   const float rep = p.repetition != nullptr ? p.repetition[row] : 1.f;
   const float freq = p.frequency != nullptr ? p.frequency[row] : 0.f;
   const float pres = p.presence != nullptr ? p.presence[row] : 0.f;
-  const T* x = p.logits + row * p.ld + v0;
-  float* y = p.out + (int64_t)row * p.vocab + v0;
-  const uint32_t* allowed = p.allowed != nullptr ? reinterpret_cast<const uint32_t*>(p.allowed) + row * p.allowed_ld : nullptr;
-  auto one = [&](float v, int i) {
-    if (with_tokens) {
-      const uint32_t c = counts[i];
-      if (c != 0) {
-        v = v > 0.f ? v / rep : v * rep;
-        const uint32_t made = c & ~kSeen;
-        if (made != 0) v = v - freq * (float)made - pres;
+  const bool counted = with_tokens || b1 > b0;
+  int hits = 0;
+  if (counted) {
+    const int bias_id = b0 + tid < b1 ? p.bias_ids[b0 + tid] - v0 : -1;
+    const float bias = b0 + tid < b1 ? p.bias_values[b0 + tid] : 0.f;
+    const bool hit = bias_id >= 0 && bias_id < here;
+#pragma unroll
+    for (int i = 0; i < kEach / 4; ++i) reinterpret_cast<uint4*>(counts)[i * kThreads + tid] = make_uint4(0, 0, 0, 0);
+    const uint32_t mask = __ballot_sync(0xffffffffu, hit);
+    if (lane == 0) warp_hits[warp] = __popc(mask);
+    __syncthreads();
+    int before = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += warp_hits[w];
+      hits += warp_hits[w];
+    }
+    if (hit) {
+      const int k = before + __popc(mask & ((1u << lane) - 1));
+      hit_ids[k] = bias_id;
+      hit_values[k] = bias;
+    }
+    if (tid < 4) hit_ids[hits + tid] = -1;
+    auto count = [&](int id, int i) {
+      const int at = id - v0;
+      if (i < n && at >= 0 && at < here) {
+        if (i >= prompt) atomicAdd(&counts[at], 1u);
+        else atomicOr(&counts[at], kSeen);
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) count(held[u], u * kThreads + tid);
+#pragma unroll 4
+    for (int i = kAhead * kThreads + tid; i < n; i += kThreads) count(ids[i], i);
+    if (hits > 0) {
+      __syncthreads();
+      if (tid < hits) {
+        const int id = hit_ids[tid];
+        int first = tid, others = 0;
+        for (int k = 0; k < hits; k += 4) {
+          const int4 h = *reinterpret_cast<const int4*>(hit_ids + k);
+          others += (h.x == id) + (h.y == id) + (h.z == id) + (h.w == id);
+          if (h.w == id) first = min(first, k + 3);
+          if (h.z == id) first = min(first, k + 2);
+          if (h.y == id) first = min(first, k + 1);
+          if (h.x == id) first = min(first, k);
+        }
+        if (first == tid) {
+          atomicOr(&counts[id], kBiased | (uint32_t)tid << kHitShift);
+          if (others > 1) {
+            float sum = 0.f;
+            for (int k = tid; k < hits; ++k)
+              if (hit_ids[k] == id) sum += hit_values[k];
+            hit_values[tid] = sum;  // no other thread sums this id
+          }
+        }
       }
     }
-    if (with_bias) v += bias[i];
-    if (allowed != nullptr && !(allowed[(v0 + i) >> 5] >> ((v0 + i) & 31) & 1)) v = -INFINITY;
+    __syncthreads();
+  }
+  auto marked = [&](float v, uint32_t c) {
+    const uint32_t made = c & kMadeMask;
+    if ((c & kSeen) || made) v = v > 0.f ? v / rep : v * rep;
+    if (made) v = v - freq * (float)made - pres;
+    if (c & kBiased) v += hit_values[c >> kHitShift & (kThreads - 1)];
     return v;
   };
-  constexpr int N = 16 / sizeof(T);  // values of one 16-byte load
-  const bool aligned = (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) % 16 == 0;
-  int done = 0;
-  if (aligned) {
-    done = here / N * N;
-    for (int i = threadIdx.x * N; i < done; i += kThreads * N) {
-      const uint4 w = *reinterpret_cast<const uint4*>(x + i);
-      const T* e = reinterpret_cast<const T*>(&w);
-      float v[N];
+  if (kAligned) {
 #pragma unroll
-      for (int u = 0; u < N; ++u) v[u] = one(to_float(e[u]), i + u);
+    for (int u = 0; u < kEach / 4; ++u) {
+      const int i = (u * kThreads + tid) * 4;
+      if (i >= here) break;
+      const T* e = reinterpret_cast<const T*>(&raw[u]);
+      float v[4] = {to_float(e[0]), to_float(e[1]), to_float(e[2]), to_float(e[3])};
+      if (counted) {
+        const uint4 c = *reinterpret_cast<const uint4*>(counts + i);
+        if (c.x | c.y | c.z | c.w) {
+          if (c.x) v[0] = marked(v[0], c.x);
+          if (c.y) v[1] = marked(v[1], c.y);
+          if (c.z) v[2] = marked(v[2], c.z);
+          if (c.w) v[3] = marked(v[3], c.w);
+        }
+      }
 #pragma unroll
-      for (int u = 0; u < N; u += 4) *reinterpret_cast<float4*>(y + i + u) = make_float4(v[u], v[u + 1], v[u + 2], v[u + 3]);
+      for (int k = 0; k < 4; ++k)
+        if (!(bits[u] >> k & 1)) v[k] = -INFINITY;
+      __stcs(reinterpret_cast<float4*>(y + i), make_float4(v[0], v[1], v[2], v[3]));
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+      const int i = u * kThreads + tid;
+      if (i >= here) break;
+      float v = to_float(single[u]);
+      if (counted && counts[i]) v = marked(v, counts[i]);
+      if (allowed != nullptr && !(allowed[i >> 5] >> (i & 31) & 1)) v = -INFINITY;
+      y[i] = v;
     }
   }
-  for (int i = done + threadIdx.x; i < here; i += kThreads) y[i] = one(to_float(x[i]), i);
+  // ---- a row with more biases than threads: kThreads more at a time, added to what has been written
+  for (int base = b0 + kThreads; base < b1; base += kThreads) {
+    __syncthreads();
+    const int many = min(kThreads, b1 - base);
+    if (tid < many) {
+      hit_ids[tid] = p.bias_ids[base + tid] - v0;
+      hit_values[tid] = p.bias_values[base + tid];
+    }
+    __syncthreads();
+    if (tid >= many) continue;
+    const int id = hit_ids[tid];
+    bool first = id >= 0 && id < here && !(allowed != nullptr && !(allowed[id >> 5] >> (id & 31) & 1));
+    for (int k = 0; first && k < tid; ++k) first = hit_ids[k] != id;
+    if (first) {
+      float sum = 0.f;
+      for (int k = tid; k < many; ++k)
+        if (hit_ids[k] == id) sum += hit_values[k];
+      y[id] += sum;
+    }
+  }
 }
 
 template <typename T>
-void launch(LogitsParams<T>& p, const at::Tensor& logits) {
-  p.logits = reinterpret_cast<const T*>(logits.data_ptr());
+cudaError_t launch(const LogitsParams& p, cudaStream_t stream) {
   const dim3 grid((unsigned)((p.vocab + kSlice - 1) / kSlice), (unsigned)p.rows);
-  process_logits_kernel<T><<<grid, kThreads, 0, at::cuda::getCurrentCUDAStream()>>>(p);
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  // Four logits at a time where every row starts on their boundary, and ends on one.
+  const bool aligned = p.vocab % 4 == 0 && p.ld % 4 == 0 && reinterpret_cast<uintptr_t>(p.logits) % (4 * sizeof(T)) == 0 &&
+                       reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+  if (aligned) process_logits_kernel<T, true><<<grid, kThreads, 0, stream>>>(p);
+  else process_logits_kernel<T, false><<<grid, kThreads, 0, stream>>>(p);
+  return cudaGetLastError();
 }
-
-const at::Tensor* given(const c10::optional<at::Tensor>& t) { return t.has_value() ? &*t : nullptr; }
 
 }  // namespace
 
-at::Tensor process_logits(at::Tensor logits, c10::optional<at::Tensor> tokens, c10::optional<at::Tensor> token_lens,
-                          c10::optional<at::Tensor> prompt_lens, c10::optional<at::Tensor> repetition,
-                          c10::optional<at::Tensor> presence, c10::optional<at::Tensor> frequency,
-                          c10::optional<at::Tensor> bias_offsets, c10::optional<at::Tensor> bias_ids,
-                          c10::optional<at::Tensor> bias_values, c10::optional<at::Tensor> allowed,
-                          c10::optional<at::Tensor> out) {
-  TORCH_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && (logits.stride(1) == 1 || logits.size(1) <= 1),
-                    "logits must be [rows, vocab] on the GPU with contiguous rows");
-  const auto type = logits.scalar_type();
-  TORCH_CHECK_VALUE(type == at::kBFloat16 || type == at::kHalf || type == at::kFloat,
-                    "logits must be bfloat16, float16 or float32");
-  const at::Device dev = logits.device();
-  const int64_t rows = logits.size(0), vocab = logits.size(1);
-  TORCH_CHECK_VALUE(rows < 65536 && vocab < (int64_t(1) << 31) - kSlice, "too many rows or too large a vocabulary");
-  auto per_row = [&](const at::Tensor* t, const char* name, at::ScalarType want, int64_t size) {
-    if (t == nullptr) return;
-    TORCH_CHECK_VALUE(t->device() == dev && t->scalar_type() == want && t->dim() == 1 && t->size(0) == size && t->is_contiguous(),
-                      name, " must be a contiguous ", want, " tensor of ", size, " on ", dev);
-  };
-  per_row(given(token_lens), "token_lens", at::kInt, rows);
-  per_row(given(prompt_lens), "prompt_lens", at::kInt, rows);
-  per_row(given(repetition), "repetition", at::kFloat, rows);
-  per_row(given(presence), "presence", at::kFloat, rows);
-  per_row(given(frequency), "frequency", at::kFloat, rows);
-  per_row(given(bias_offsets), "the bias offsets", at::kInt, rows + 1);
-  if (tokens.has_value()) {
-    TORCH_CHECK_VALUE(tokens->device() == dev && tokens->scalar_type() == at::kInt && tokens->dim() == 2 &&
-                          tokens->size(0) == rows && (tokens->stride(1) == 1 || tokens->size(1) <= 1) &&
-                          tokens->size(1) < (int64_t(1) << 31) - kThreads,
-                      "tokens must be int32 [rows, history] on ", dev, " with contiguous rows");
-  } else {
-    TORCH_CHECK_VALUE(!token_lens.has_value() && !prompt_lens.has_value() && !repetition.has_value() &&
-                          !presence.has_value() && !frequency.has_value(),
-                      "lengths and penalties need tokens");
-  }
-  TORCH_CHECK_VALUE(bias_offsets.has_value() == bias_ids.has_value() && bias_ids.has_value() == bias_values.has_value(),
-                    "bias is (offsets, ids, values)");
-  if (bias_ids.has_value()) {
-    TORCH_CHECK_VALUE(bias_ids->size(0) < (int64_t(1) << 31) - 64, "too many biases");
-    per_row(given(bias_ids), "the bias ids", at::kInt, bias_ids->numel());
-    per_row(given(bias_values), "the bias values", at::kFloat, bias_ids->numel());
-  }
-  if (allowed.has_value()) {
-    TORCH_CHECK_VALUE(allowed->device() == dev && allowed->scalar_type() == at::kInt && allowed->dim() == 2 &&
-                          allowed->size(0) == rows && allowed->size(1) == (vocab + 31) / 32 &&
-                          (allowed->stride(1) == 1 || allowed->size(1) <= 1),
-                      "allowed must be int32 [rows, ceil(vocab / 32)] on ", dev, " with contiguous rows");
-  }
-  c10::cuda::CUDAGuard guard(dev);
-  at::Tensor y;
-  if (out.has_value()) {
-    TORCH_CHECK_VALUE(out->device() == dev && out->scalar_type() == at::kFloat && out->is_contiguous() &&
-                          out->sizes() == logits.sizes(),
-                      "out must be contiguous float32 of the logits' shape on ", dev);
-    TORCH_CHECK_VALUE(out->data_ptr() != logits.data_ptr() || (type == at::kFloat && logits.is_contiguous()),
-                      "out may be the logits only where they are contiguous float32");
-    y = *out;
-  } else {
-    y = at::empty({rows, vocab}, logits.options().dtype(at::kFloat));
-  }
-  if (rows == 0 || vocab == 0) return y;
-  auto fill = [&](auto& p) {
-    p.ld = logits.stride(0);
-    p.out = y.data_ptr<float>();
-    p.rows = (int)rows, p.vocab = (int)vocab;
-    if (tokens.has_value()) {
-      p.tokens = tokens->data_ptr<int>();
-      p.tokens_ld = tokens->stride(0);
-      p.tokens_width = (int)tokens->size(1);
-    }
-    auto ints = [](const c10::optional<at::Tensor>& t) { return t.has_value() ? t->data_ptr<int>() : nullptr; };
-    auto floats = [](const c10::optional<at::Tensor>& t) { return t.has_value() ? t->data_ptr<float>() : nullptr; };
-    p.token_lens = ints(token_lens), p.prompt_lens = ints(prompt_lens);
-    p.repetition = floats(repetition), p.presence = floats(presence), p.frequency = floats(frequency);
-    p.bias_offsets = ints(bias_offsets), p.bias_ids = ints(bias_ids), p.bias_values = floats(bias_values);
-    p.bias_count = bias_ids.has_value() ? (int)bias_ids->numel() : 0;
-    p.allowed = ints(allowed);
-    p.allowed_ld = allowed.has_value() ? allowed->stride(0) : 0;
-  };
-  if (type == at::kBFloat16) {
-    LogitsParams<__nv_bfloat16> p{};
-    fill(p);
-    launch(p, logits);
-  } else if (type == at::kHalf) {
-    LogitsParams<__half> p{};
-    fill(p);
-    launch(p, logits);
-  } else {
-    LogitsParams<float> p{};
-    fill(p);
-    launch(p, logits);
-  }
-  return y;
+namespace mimir {
+cudaError_t launch_process_logits(const LogitsParams& p, LogitsType type, cudaStream_t stream) {
+  if (type == kLogitsFloat) return launch<float>(p, stream);
+  return type == kLogitsHalf ? launch<__half>(p, stream) : launch<__nv_bfloat16>(p, stream);
 }
+}  // namespace mimir

@@ -35,6 +35,7 @@ class _CountingModule:
             self.launches += per_call
             return fn(*args, **kwargs)
         counted.__name__ = name
+        self.__dict__[name] = counted  # later calls find it without __getattr__
         return counted
 
 

@@ -12,7 +12,7 @@ NVCC_FLAGS = ["-O3", "-std=c++17", "-gencode", "arch=compute_100a,code=sm_100a",
 if os.environ.get("MIMIR_PTXAS_VERBOSE") == "1":
     NVCC_FLAGS += ["-Xptxas", "-v"]
 
-sources = sorted(glob.glob(os.path.join("csrc", "*.cu"))) + ["csrc/bindings.cpp"]
+sources = sorted(glob.glob(os.path.join("csrc", "*.cu"))) + sorted(glob.glob(os.path.join("csrc", "*.cpp")))
 # Link the system's shared libstdc++ (the one torch itself uses).  Where the compiler's own
 # unversioned libstdc++.so link is missing, the linker would otherwise fall back to the static
 # archive and every extension would carry a private copy of the C++ runtime (its stream/locale
