@@ -90,7 +90,7 @@ std::vector<at::Tensor> invocation_gate_bwd(at::Tensor dout, at::Tensor pre, at:
 at::Tensor goldfish_mask(at::Tensor inputs, at::Tensor supervised, at::Tensor cu_seqlens, int64_t k,
                          int64_t context_width, int64_t seed, std::vector<int64_t> mix);
 int64_t embed_status(int64_t device);
-// kv_cache.cu
+// serving.cpp
 at::Tensor cache_append(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor cos, at::Tensor sin, at::Tensor pages,
                         at::Tensor scales, at::Tensor table, at::Tensor lens, at::Tensor seqs, at::Tensor cu_new);
 at::Tensor cache_reserve(at::Tensor table, at::Tensor lens, at::Tensor refs, at::Tensor seqs, at::Tensor counts,
@@ -102,11 +102,9 @@ void cache_copy(at::Tensor pages, at::Tensor scales, at::Tensor src, at::Tensor 
 at::Tensor cache_compact(at::Tensor pages, at::Tensor scales, at::Tensor table, at::Tensor refs, at::Tensor out_pages,
                          at::Tensor out_scales, at::Tensor out_table, at::Tensor out_refs);
 int64_t cache_status(int64_t device);
-// cache_attention.cu
 at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at::Tensor table, at::Tensor lens,
                            at::Tensor seqs, at::Tensor cu_new, c10::optional<at::Tensor> prefix_lens,
-                           double softmax_scale, int64_t max_new);
-// logits.cu
+                           double softmax_scale, int64_t max_new, int64_t kernel);
 at::Tensor process_logits(at::Tensor logits, c10::optional<at::Tensor> tokens, c10::optional<at::Tensor> token_lens,
                           c10::optional<at::Tensor> prompt_lens, c10::optional<at::Tensor> repetition,
                           c10::optional<at::Tensor> presence, c10::optional<at::Tensor> frequency,
@@ -189,6 +187,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cache_copy", &cache_copy);
   m.def("cache_compact", &cache_compact);
   m.def("cache_status", &cache_status);
-  m.def("cache_attention", &cache_attention);
+  m.def("cache_attention", &cache_attention, py::arg("q"), py::arg("pages"), py::arg("scales"), py::arg("page_table"),
+        py::arg("seq_lens"), py::arg("seqs"), py::arg("cu_new"), py::arg("prefix_lens"), py::arg("softmax_scale"),
+        py::arg("max_new"), py::arg("kernel") = 0);
   m.def("process_logits", &process_logits);
 }

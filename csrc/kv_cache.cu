@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) cache_append_kernel(const A
               page = -1;
             }
           }
-        } else if (first >= 0) {  // its rows become zeros
+        } else if (first >= 0 && j >= 0) {  // its rows become zeros
           rows = min(max(count - j * kCacheBlock, 0), kCacheBlock);
           row = first + j * kCacheBlock;
           if (rows > 0) report(p.status, good ? kCacheBadLength : kCacheBadSlot);

@@ -118,6 +118,22 @@ CUtensorMap pages_map(const at::Tensor& pages, int64_t keys) {
   return map;
 }
 
+// Query rows [tokens, H, 128]: boxes of 128 / group tokens, the heads of a group, 64 dimensions.
+CUtensorMap queries_map(const at::Tensor& q, int64_t group) {
+  bind_device_context();
+  CUtensorMap map;
+  cuuint64_t dims[3] = {(cuuint64_t)kCacheDim, (cuuint64_t)q.size(1), (cuuint64_t)q.size(0)};
+  cuuint64_t strides[2] = {(cuuint64_t)(q.stride(1) * 2), (cuuint64_t)(q.stride(0) * 2)};
+  cuuint32_t box[3] = {64, (cuuint32_t)group, (cuuint32_t)(128 / group)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const auto type = q.scalar_type() == at::kBFloat16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  CUresult r = tensor_map_encoder()(&map, type, 3, q.data_ptr(), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (queries) failed with code ", (int)r);
+  return map;
+}
+
 // Counters that are zero before and after every call: kept per stream, whose calls follow one another;
 // a graph, which may run beside its stream, gets its own from its pool.
 int* arrival_counters(const at::Device& dev, cudaStream_t stream, at::Tensor& keep) {
@@ -301,9 +317,10 @@ at::Tensor cache_compact(at::Tensor pages, at::Tensor scales, at::Tensor table, 
   return work.narrow(0, 0, 1);
 }
 
+// kernel: 0 chooses; 1 is the kernel that splits the keys, 2 the one for prompts.
 at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at::Tensor table, at::Tensor lens,
                            at::Tensor seqs, at::Tensor cu_new, c10::optional<at::Tensor> prefix_lens,
-                           double softmax_scale, int64_t max_new) {
+                           double softmax_scale, int64_t max_new, int64_t kernel) {
   check_pool(pages, scales, 0);
   const at::Device dev = pages.device();
   check_rows(q, "q", dev);
@@ -321,7 +338,6 @@ at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at
   const int64_t n = seqs.size(0);
   if (q.size(0) == 0) return out;
   if (n == 0 || pages.size(0) == 0) return out.zero_();
-  const CUtensorMap map = pages_map(pages, kAttentionKeys);
   AttentionParams p{};
   p.q = q.data_ptr();
   p.q_tok = q.stride(0), p.q_head = q.stride(1);
@@ -334,6 +350,25 @@ at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at
   p.scale_log2 = (float)(softmax_scale * 1.4426950408889634);
   p.status = status_word(dev);
   auto stream = at::cuda::getCurrentCUDAStream();
+  const bool bf16 = q.scalar_type() == at::kBFloat16;
+  // (q strides of zero, a broadcast, are not for a tensor map)
+  const int64_t most_rows = (max_new < 1 ? q.size(0) : std::min(max_new, q.size(0))) * p.group;
+  const int64_t tiles = (q.size(0) * p.group / 256 + n) * KV;
+  const bool can = p.group <= 64 && p.scale_log2 > 0.f && q.stride(0) > 0 && q.stride(1) > 0;
+  SERVING_CHECK(kernel != 2 || can, "the prompt kernel cannot take these arguments");
+  if (kernel == 2 || (kernel == 0 && can && most_rows >= 64 && tiles >= 74)) {
+    const CUtensorMap map_q = queries_map(q, p.group), map_pages = pages_map(pages, kPromptKeys);
+    for (int64_t base = 0; base < n; base += kAttentionSeqs) {
+      p.n = (int)std::min<int64_t>(kAttentionSeqs, n - base);
+      p.seqs = seqs.data_ptr<int>() + base;
+      p.cu = cu_new.data_ptr<int>() + base;
+      p.prefix = prefix_lens.has_value() ? prefix_lens->data_ptr<int>() + base : nullptr;
+      p.last_batch = base + p.n == n;
+      C10_CUDA_CHECK(launch_cache_prompt(map_q, map_pages, p, bf16, stream));
+    }
+    return out;
+  }
+  const CUtensorMap map = pages_map(pages, kAttentionKeys);
   at::Tensor keep;
   p.arrived = arrival_counters(dev, stream, keep);
   const bool full = max_new < 1 || max_new * p.group > 8;
@@ -350,7 +385,7 @@ at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at
     at::Tensor work = at::empty({grid * (int64_t)(2 * kAttentionRows * (kCacheDim + 2))}, q.options().dtype(at::kFloat));
     p.parts = work.data_ptr<float>();
     p.part_ml = reinterpret_cast<float2*>(p.parts + (int64_t)grid * 2 * kAttentionRows * kCacheDim);
-    C10_CUDA_CHECK(launch_cache_attention(map, p, q.scalar_type() == at::kBFloat16, full, grid, stream));
+    C10_CUDA_CHECK(launch_cache_attention(map, p, bf16, full, grid, stream));
   }
   return out;
 }

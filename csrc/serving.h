@@ -109,6 +109,12 @@ struct AttentionParams {
 cudaError_t launch_cache_attention(const CUtensorMap& map, const AttentionParams& p, bool bf16, bool full, int grid,
                                    cudaStream_t stream);
 
+// ---------------------------------------------------------------- cache_prompt.cu
+constexpr int kPromptKeys = 128;  // keys of a tile: the box of the map of the pages
+// map_q: [tokens, H, 128] with boxes of 128 / group tokens, `group` heads and 64 dimensions.
+cudaError_t launch_cache_prompt(const CUtensorMap& map_q, const CUtensorMap& map_pages, const AttentionParams& p, bool bf16,
+                                cudaStream_t stream);
+
 // ---------------------------------------------------------------- logits.cu
 enum LogitsType { kLogitsFloat, kLogitsHalf, kLogitsBFloat16 };
 struct LogitsParams {

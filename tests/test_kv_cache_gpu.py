@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from mimir_b200 import ops
-from mimir_b200.ops._ext import KernelTimeout, check_kernel_status, kernel_status
+from mimir_b200.ops._ext import KernelTimeout, check_kernel_status, ext, kernel_status
 from mimir_b200.ops.kv_cache import BLOCK, cache_append_reference, cache_values
 from mimir_b200.ops.logits import process_logits_reference
 
@@ -50,7 +50,7 @@ def attention64(q, st, seqs, counts, prefix=None, softmax_scale=DIM ** -0.5, p_b
     kv = st["pages"].shape[2]
     out = torch.zeros_like(q, dtype=torch.float64)
     bound = torch.zeros_like(out)
-    unit = 2.0 ** -9 if q.dtype == torch.bfloat16 else 2.0 ** -12
+    unit = 2.0 ** -8 if q.dtype == torch.bfloat16 else 2.0 ** -11  # half a step of 8 or 11 significant bits
     row = 0
     for i, (slot, count) in enumerate(zip(seqs, counts)):
         n = int(st["lens"][slot])
@@ -77,16 +77,24 @@ def attention64(q, st, seqs, counts, prefix=None, softmax_scale=DIM ** -0.5, p_b
     return out, bound + 1e-30
 
 
+def attend(q, st, seqs, cu, prefix=None, softmax_scale=None, max_new=None, kernel=0):
+    """``ops.cache_attention``, or with ``kernel`` one of its two kernels whatever the sizes."""
+    args = (q, st["pages"], st["scales"], st["table"], st["lens"], ints(seqs).to(DEV), ints(cu).to(DEV),
+            None if prefix is None else ints(prefix).to(DEV))
+    if kernel:
+        return ext().cache_attention(*args, softmax_scale or DIM ** -0.5, max_new or 0, kernel)
+    return ops.cache_attention(*args, max_new=max_new, softmax_scale=softmax_scale)
+
+
 def check_attention(st, seqs, counts, heads, dtype=torch.bfloat16, prefix=None, seed=5, extra_rows=0, max_new=None, q=None,
-                    softmax_scale=None):
+                    softmax_scale=None, kernel=0):
     gen = torch.Generator(DEV).manual_seed(seed)
     total = sum(counts)
     if q is None:
         q = (1.5 * torch.randn(total + extra_rows, heads, DIM, generator=gen, device=DEV)).to(dtype)
-    cu = ints([sum(counts[:i]) for i in range(len(counts) + 1)]).to(DEV)
-    out = ops.cache_attention(q, st["pages"], st["scales"], st["table"], st["lens"], ints(seqs).to(DEV), cu,
-                              None if prefix is None else ints(prefix).to(DEV), max_new=max_new, softmax_scale=softmax_scale)
-    ref, bound = attention64(q, st, seqs, counts, prefix, softmax_scale or DIM ** -0.5, p_bits=8)
+    cu = [sum(counts[:i]) for i in range(len(counts) + 1)]
+    out = attend(q, st, seqs, cu, prefix, softmax_scale, max_new, kernel)
+    ref, bound = attention64(q, st, seqs, counts, prefix, softmax_scale or DIM ** -0.5, p_bits=11)
     check_kernel_status(DEV)
     assert out.dtype == q.dtype and out.shape == q.shape and torch.isfinite(out).all()
     err = (out.double() - ref).abs()
@@ -108,7 +116,8 @@ def test_single_tokens_at_every_edge(page):
 def test_head_groups_and_types(heads, kv, dtype):
     st = filled([70, 9, 300], kv, 32, seed=heads)
     check_attention(st, [2, 0, 1], [1, 1, 1], heads, dtype, max_new=1)
-    check_attention(st, [2, 0, 1], [5, 70, 2], heads, dtype, max_new=70)
+    for kernel in (0, 1, 2):
+        check_attention(st, [2, 0, 1], [5, 70, 2], heads, dtype, max_new=70, kernel=kernel)
 
 
 @pytest.mark.parametrize("counts", [[2, 3, 1, 4], [0, 17, 0, 33], [64, 65, 1, 200], [300, 1, 129, 256]])
@@ -117,8 +126,8 @@ def test_several_tokens_and_prefixes(counts, prefix):
     lens = [c + old for c, old in zip(counts, [5, 0, 700, 0])]
     st = filled(lens, 2, 64, seed=sum(counts))
     p = None if prefix is None else [n if prefix == "all" else n // 2 for n in lens]
-    check_attention(st, [0, 1, 2, 3], counts, 8, prefix=p, extra_rows=3)
-    check_attention(st, [0, 1, 2, 3], counts, 8, prefix=p, extra_rows=3, max_new=max(counts))
+    for kernel in (0, 1, 2):
+        check_attention(st, [0, 1, 2, 3], counts, 8, prefix=p, extra_rows=3, max_new=max(counts), kernel=kernel)
 
 
 def test_a_long_sequence_is_split_and_many_short_ones_are_not():
@@ -127,6 +136,22 @@ def test_a_long_sequence_is_split_and_many_short_ones_are_not():
     lens = [1 + i % 7 for i in range(1500)]  # more sequences than one launch takes
     st = filled(lens, 1, 16)
     check_attention(st, list(range(1500)), [1] * 1500, 2, max_new=1)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+def test_prompts_at_every_edge(page):
+    """The prompt kernel: lengths and new tokens around its tiles of 128 keys and 32 tokens, many sequences."""
+    counts = [1, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200, 0, 511, 1, 300]
+    old = [0, 0, 1, 200, 0, 64, 0, 128, 0, 1, 57, 5, 1, 1000, 0]
+    st = filled([c + o for c, o in zip(counts, old)], 5, page, seed=page)
+    for prefix in (None, [c + o for c, o in zip(counts, old)], [7 * i for i in range(15)]):
+        check_attention(st, list(range(15)), counts, 20, prefix=prefix, extra_rows=2, kernel=2)
+
+
+def test_many_short_prompts():
+    counts = [1 + (i * 7) % 50 for i in range(1100)]  # more sequences than one launch takes
+    st = filled(counts, 1, 16)
+    check_attention(st, list(range(1100)), counts, 4, kernel=2)
 
 
 def test_results_do_not_depend_on_the_run():
@@ -141,7 +166,8 @@ def test_value_scales_far_apart():
     st = filled([500, 33], 1, 16, spread=10.0)
     st["scales"][:, 0] = 2.0 ** -7  # keys as usual
     check_attention(st, [0, 1], [1, 1], 4, max_new=1)
-    check_attention(st, [0, 1], [40, 33], 4, max_new=40)
+    for kernel in (1, 2):
+        check_attention(st, [0, 1], [40, 33], 4, max_new=40, kernel=kernel)
 
 
 def test_queries_of_any_size_and_a_scale_of_ones_own():
@@ -149,22 +175,27 @@ def test_queries_of_any_size_and_a_scale_of_ones_own():
     gen = torch.Generator(DEV).manual_seed(1)
     q = torch.randn(2, 8, DIM, generator=gen, device=DEV)
     for factor, scale in ((2.0 ** 20, DIM ** -0.5 * 2.0 ** -20), (2.0 ** -30, DIM ** -0.5 * 2.0 ** 30), (1.0, 0.0)):
-        check_attention(st, [0, 1], [1, 1], 8, q=(q * factor).bfloat16(), softmax_scale=scale or 1e-9)
+        for kernel in (1, 2):
+            check_attention(st, [0, 1], [1, 1], 8, q=(q * factor).bfloat16(), softmax_scale=scale or 1e-9, kernel=kernel)
 
 
 def test_strided_queries():
     st = filled([50, 90], 2, 32)
     packed = torch.randn(9, 20, DIM, device=DEV).bfloat16()
-    check_attention(st, [0, 1], [4, 5], 8, q=packed[:, 7:15])
     wide = torch.randn(8, 9, 2 * DIM, device=DEV).half().transpose(0, 1)
-    check_attention(st, [0, 1], [4, 5], 8, q=wide[..., :DIM])
+    for kernel in (1, 2):
+        check_attention(st, [0, 1], [4, 5], 8, q=packed[:, 7:15], kernel=kernel)
+        check_attention(st, [0, 1], [4, 5], 8, q=wide[..., :DIM], kernel=kernel)
+    one = torch.randn(1, 8, DIM, device=DEV).bfloat16().expand(9, 8, DIM)
+    check_attention(st, [0, 1], [4, 5], 8, q=one)
 
 
-def test_bytes_beyond_the_length_do_not_matter():
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_bytes_beyond_the_length_do_not_matter(kernel):
     """NaN bytes, NaN scales and pages of others behind a sequence's end, and in pages that it does not hold."""
     for lens, counts in (([1, 17, 70], [1, 1, 1]), ([40, 150, 70], [33, 130, 2])):
         st = filled(lens, 2, 64, seed=3)
-        q, want = check_attention(st, [0, 1, 2], counts, 8)
+        q, want = check_attention(st, [0, 1, 2], counts, 8, kernel=kernel)
         nan = torch.tensor(0x7F, dtype=torch.uint8, device=DEV)
         held = torch.zeros(st["pages"].shape[0], dtype=torch.bool, device=DEV)
         for i, n in enumerate(lens):
@@ -175,33 +206,31 @@ def test_bytes_beyond_the_length_do_not_matter():
             st["scales"][row[-1], :, :, -(-inside // BLOCK):] = math.nan
         st["pages"].view(torch.uint8)[~held] = nan
         st["scales"][~held] = math.nan
-        cu = ints([0, counts[0], sum(counts[:2]), sum(counts)]).to(DEV)
-        got = ops.cache_attention(q, st["pages"], st["scales"], st["table"], st["lens"], ints([0, 1, 2]).to(DEV), cu)
+        got = attend(q, st, [0, 1, 2], [0, counts[0], sum(counts[:2]), sum(counts)], kernel=kernel)
         assert torch.equal(got, want)
 
 
 @pytest.mark.parametrize("which", [0, 1])
-@pytest.mark.parametrize("count", [3, 60])
-def test_a_poisoned_block_reaches_the_rows_that_see_it(which, count):
+@pytest.mark.parametrize("count,kernel", [(3, 1), (60, 1), (3, 2), (60, 2)])
+def test_a_poisoned_block_reaches_the_rows_that_see_it(which, count, kernel):
     n = 100
     st = filled([n, 30], 2, 32)
-    q, want = check_attention(st, [0, 1], [count, 1], 8)
+    q, want = check_attention(st, [0, 1], [count, 1], 8, kernel=kernel)
     at = 98  # the block of tokens 96..99
     st["scales"][st["table"][0, at // 32].long(), which, 1, at % 32 // BLOCK] = math.nan
-    got = ops.cache_attention(q, st["pages"], st["scales"], st["table"], st["lens"], ints([0, 1]).to(DEV),
-                              ints([0, count, count + 1]).to(DEV))
+    got = attend(q, st, [0, 1], [0, count, count + 1], kernel=kernel)
     hit = torch.zeros(count + 1, 8, dtype=torch.bool, device=DEV)
     hit[max(0, 96 - (n - count)):count, 4:] = True  # heads of the second key/value head, from position 96 on
     assert torch.equal(torch.isnan(got).all(-1), hit) and torch.equal(torch.isnan(got).any(-1), hit)
     assert torch.equal(got[~hit], want[~hit])
 
 
-def test_rows_without_keys_are_zero():
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_rows_without_keys_are_zero(kernel):
     st = filled([10, 20], 1, 16)
     st["lens"][0] = 0  # an emptied slot that is still asked for
     q = torch.randn(4, 2, DIM, device=DEV).bfloat16()
-    out = ops.cache_attention(q, st["pages"], st["scales"], st["table"], st["lens"], ints([0, 1]).to(DEV),
-                              ints([0, 1, 2]).to(DEV))
+    out = attend(q, st, [0, 1], [0, 1, 2], kernel=kernel)
     assert not out[0].any() and out[1].any() and not out[2:].any()
     with pytest.raises(KernelTimeout, match="kv_cache"):  # fewer tokens than new ones: reported
         check_kernel_status(DEV)
@@ -219,7 +248,8 @@ def test_offsets_beyond_32_bits():
     x = (100 * torch.randn(3, 2, kv, page, DIM, device=DEV, generator=torch.Generator(DEV).manual_seed(0))).clamp(-448, 448)
     st["pages"].view(torch.uint8)[st["table"][0].long()] = x.to(torch.float8_e4m3fn).view(torch.uint8)
     check_attention(st, [0], [1], 8, max_new=1)
-    check_attention(st, [0], [300], 8, max_new=300)
+    for kernel in (1, 2):
+        check_attention(st, [0], [300], 8, max_new=300, kernel=kernel)
     cos, sin = tables(1024, DIM)
     k = torch.randn(700, kv, DIM, device=DEV).bfloat16()
     ops.cache_append(k, k, k, cos.to(DEV), sin.to(DEV), st["pages"], st["scales"], st["table"], st["lens"],
