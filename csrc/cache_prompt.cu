@@ -26,6 +26,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "serving.h"
 
@@ -129,6 +131,28 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& lo, uint32_t& hi) { 
   asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
       : "=r"(lo), "=r"(hi)
       : "r"(w));
+}
+// Two fp32 values in one register pair: products, sums and the like of both at once.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void split_pair(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 template <bool kBf16>
 __device__ __forceinline__ float2 unpack(uint32_t w) {
@@ -466,56 +490,67 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 32; ++i) sv[c * 32 + i] = __uint_as_float(raw[c][i]);
       }
       const int rel = lim - j * kTile;  // columns below it are seen
-      const bool edge = (j + 1) * kTile > min_lim;
-      if (edge) {
-#pragma unroll
-        for (int c = 0; c < 128; ++c) sv[c] = c >= rel ? -INFINITY : sv[c];
-      }
-      const float2* sc = reinterpret_cast<const float2*>(scale_ring + (j % kScaleRing) * 16);
-      float mx = kLowest;
-#pragma unroll
-      for (int y = 0; y < 8; ++y) {
-        float t[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = sv[y * 16 + e];
-#pragma unroll
-        for (int c = 4; c < 16; c += 4)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) t[e] = fmaxf(t[e], sv[y * 16 + c + e]);
-        const float2 kv = sc[y];
-        const float ev = kv.y == kv.y ? (float)((__float_as_int(kv.y) >> 23) - 127) : kv.y;
-        mx = fmaxf(mx, fmaf(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])), factor * kv.x, ev));
-      }
+      const float4* sc = reinterpret_cast<const float4*>(scale_ring + (j % kScaleRing) * 16);
       float alpha = 1.f;
       bool rescale = false;
-      if (mx > M + kRescaleThreshold) {
-        alpha = fast_exp2(M - mx);
-        rescale = j > 0;
-        M = mx;
-      }
-      l *= alpha;
       uint32_t pk[64];
+      // Tiles that some row sees only in part are masked; the others do without those instructions.
+      auto probabilities = [&](auto masked) {
+        constexpr bool kMasked = decltype(masked)::value;
+        if (kMasked) {
 #pragma unroll
-      for (int y = 0; y < 8; ++y) {
-        const float2 kv = sc[y];
-        const float ev = kv.y == kv.y ? (float)((__float_as_int(kv.y) >> 23) - 127) : kv.y;
-        const float mult = factor * kv.x, add = ev - M;
-        const float inv = __int_as_float(0x7f000000 - __float_as_int(kv.y));  // 1 / scale
-        float sum[2] = {0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const int col = y * 16 + 2 * c;
-          float a = fast_exp2(fmaf(sv[col], mult, add)), d = fast_exp2(fmaf(sv[col + 1], mult, add));
-          if (edge) {  // also beside a poisoned block's NaN
-            if (col >= rel) a = 0.f;
-            if (col + 1 >= rel) d = 0.f;
-          }
-          sum[0] += a, sum[1] += d;
-          pk[y * 8 + c] = half2_bits(a, d);
+          for (int c = 0; c < 128; ++c) sv[c] = c >= rel ? -INFINITY : sv[c];
         }
-        const float both = sum[0] + sum[1];
-        if (both != 0.f) l = fmaf(both, kv.y == kv.y ? inv : kv.y, l);  // a block that is not seen adds nothing
-      }
+        float mult[8], ev[8], inv[8];  // of the blocks: the scores' factor, log2 of the values' scale, its inverse
+#pragma unroll
+        for (int y = 0; y < 8; y += 2) {
+          const float4 two = sc[y / 2];
+          mult[y] = factor * two.x, mult[y + 1] = factor * two.z;
+          // NaN stays NaN
+          ev[y] = two.y == two.y ? (float)((__float_as_int(two.y) >> 23) - 127) : two.y;
+          ev[y + 1] = two.w == two.w ? (float)((__float_as_int(two.w) >> 23) - 127) : two.w;
+          inv[y] = two.y == two.y ? __int_as_float(0x7f000000 - __float_as_int(two.y)) : two.y;
+          inv[y + 1] = two.w == two.w ? __int_as_float(0x7f000000 - __float_as_int(two.w)) : two.w;
+        }
+        float mx = kLowest;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const float* v = sv + y * 16;
+          const float t0 = max3(v[0], v[1], v[2]), t1 = max3(v[3], v[4], v[5]), t2 = max3(v[6], v[7], v[8]);
+          const float t3 = max3(v[9], v[10], v[11]), t4 = max3(v[12], v[13], v[14]);
+          mx = fmaxf(mx, fmaf(max3(max3(t0, t1, t2), max3(t3, t4, v[15]), t0), mult[y], ev[y]));
+        }
+        if (mx > M + kRescaleThreshold) {
+          alpha = fast_exp2(M - mx);
+          rescale = j > 0;
+          M = mx;
+        }
+        l *= alpha;
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+          const uint64_t m2 = pair_of(mult[y], mult[y]), a2 = pair_of(ev[y] - M, ev[y] - M);
+          uint64_t sum = pair_of(0.f, 0.f);
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            const int col = y * 16 + 2 * c;
+            float a, d;
+            split_pair(fma_pair(pair_of(sv[col], sv[col + 1]), m2, a2), a, d);
+            a = fast_exp2(a), d = fast_exp2(d);
+            if (kMasked) {  // also beside a poisoned block's NaN
+              if (col >= rel) a = 0.f;
+              if (col + 1 >= rel) d = 0.f;
+            }
+            sum = add_pair(sum, pair_of(a, d));
+            pk[y * 8 + c] = half2_bits(a, d);
+          }
+          float s0, s1;
+          split_pair(sum, s0, s1);
+          const float both = s0 + s1;
+          if (!kMasked || both != 0.f) l = fmaf(both, inv[y], l);  // a block that is not seen adds nothing
+        }
+      };
+      if ((j + 1) * kTile > min_lim) probabilities(std::true_type{});
+      else probabilities(std::false_type{});
       // P_x(j) overwrites the columns that PV_x(j-1) reads, and a rescale touches O_x: both wait for it.
       if (j > 0) {
         ok = warp_wait(&bar->o_done[x], (j - 1) & 1, status, kCacheTimeout);
