@@ -10,8 +10,9 @@
 //
 //   producer warp:  128 keys and values as bytes by TMA, page by page
 //   convert warps:  bytes -> fp16, exact, into the operands' swizzled layout (two stages)
-//   MMA warp:       S_A S_B | PV_A S_A' | PV_B S_B' | ...
-//   softmax warps:  a thread has a row of 128 scores; P goes back into the first half of S
+//   MMA warps:      one a row tile: S of 64 keys, two ahead of the softmax; then, for every P that
+//                   comes, O += P V and the S after the next
+//   softmax warps:  a thread has a row of 64 scores; P goes back into the first half of its S
 //
 // The scales, powers of two of 16 keys each, stay outside the products: a key block's multiplies its
 // scores, a value block's enters the exponent, p = exp2(x + ev - M) with M the maximum of x + ev, so that
@@ -19,10 +20,13 @@
 // takes each block's sum times 2^-ev in fp32.  Query rows are shifted by a power of two into fp16's
 // range first, so that bf16 rows keep all their bits.
 //
-// TMEM (512 columns): S_A [0,128), S_B [128,256), O_A [256,384), O_B [384,512); P_X is packed fp16 in the
-// first 64 columns of S_X and read from there as the A operand of O_X += P_X V.  O is rescaled only
-// when a row's maximum grows by more than 2^8.  Registers: 512 threads start with 128 each; the
-// softmax groups take 184, the converters keep 88 and the producer and MMA group 56 (the sum is the same).
+// TMEM (512 columns): S_X0 and S_X1, 64 columns each, for tiles A and B, then O_A and O_B, 128 each; P is
+// packed fp16 in the first 32 columns of its S and read from there as the A operand.  With one S of
+// 128 keys a tile (the same columns), scores to P to products is a chain that leaves the tensor
+// cores idle for more than half of the time; with two of 64 the next scores are there when a softmax ends.
+// O is rescaled only when a row's maximum grows by more than 2^8; only then is the last product
+// waited for.  Registers: 512 threads start with 128 each; the softmax groups take 184, the converters
+// keep 88 and the producer and MMA group 56 (the sum is the same).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -36,6 +40,7 @@ using namespace mimir;
 namespace {
 
 constexpr int kTile = 128;
+constexpr int kHalf = 64;                               // keys of a turn
 constexpr int kThreads = 512;
 constexpr uint32_t kTileBytes = kTile * kCacheDim * 2;  // 32 KB of fp16
 constexpr uint32_t kChunkBytes = kTileBytes / 2;        // one half of 64 dimensions
@@ -50,8 +55,9 @@ struct __align__(8) Barriers {
   uint64_t raw_empty[2];
   uint64_t scales_full[kScaleRing];
   uint64_t k_full[2], v_full[2]; // converted
-  uint64_t kv_empty[2];
-  uint64_t s_full[2], p_full[2], o_done[2];  // per row tile
+  uint64_t k_empty[2], v_empty[2];
+  uint64_t s_full[2][2], p_full[2][2];  // per row tile and buffer
+  uint64_t o_done[2];                   // per row tile
   uint64_t mma_done;
   uint32_t tmem_base;
   int pad;
@@ -61,7 +67,7 @@ constexpr uint32_t kSmemKV = 2 * kTileBytes;                 // stage s: K at +2
 constexpr uint32_t kSmemRaw = 6 * kTileBytes;                // K bytes, V bytes
 constexpr uint32_t kSmemScales = kSmemRaw + 2 * kRawBytes;   // [kScaleRing][8 blocks][k, v]
 constexpr uint32_t kSmemBar = kSmemScales + kScaleRing * 16 * sizeof(float);
-constexpr uint32_t kSmemBytes = kSmemBar + sizeof(Barriers) + 1024;
+constexpr uint32_t kSmemBytes = kSmemBar + sizeof(Barriers);
 static_assert(kSmemBytes <= 232448, "shared memory of a block");
 
 __device__ __forceinline__ uint8_t* q_tile(uint8_t* b, int x) { return b + x * kTileBytes; }
@@ -73,13 +79,24 @@ __device__ __forceinline__ uint8_t* raw_buffer(uint8_t* b, int kv) { return b + 
 __host__ __device__ constexpr uint32_t idesc_f16_f32(int M, int N, int b_mn) {
   return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
-// D[tmem] (+)= A[tmem] * B[smem]
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
+// Issued by the lane for which `leader` holds; the whole warp goes through the code, so that operands stay
+// in uniform registers.  D[tmem] (+)= A[smem] * B[smem], D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t leader) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc)
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc, uint32_t leader) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc), "r"(leader)
       : "memory");
 }
 __device__ __forceinline__ void tmem_ld32_nowait(uint32_t taddr, uint32_t (&r)[32]) {
@@ -144,11 +161,6 @@ __device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c)
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -167,11 +179,14 @@ template <bool kBf16>
 __global__ void __launch_bounds__(kThreads, 1)
     cache_prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_pages,
                         const AttentionParams p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];  // what the swizzle needs
+  if (smem_u32(smem) & 1023) {
+    if (threadIdx.x == 0) record_status(p.status, kCacheTimeout);
+    return;
+  }
   Barriers* bar = reinterpret_cast<Barriers*>(smem + kSmemBar);
   float* scale_ring = reinterpret_cast<float*>(smem + kSmemScales);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // uniform
   const int kvh = blockIdx.x % p.KV, group = p.group;
   const int tokens = kTile / group, per = 2 * tokens;  // tokens of a tile, and of this block
 
@@ -223,9 +238,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     return max(min(lim, len), 0);
   };
   const bool has_b = tok0 + tokens < count;
-  const int nkv_a = (limit_of(min(tok0 + tokens, count) - 1) + kTile - 1) / kTile;
-  const int nkv_b = has_b ? (limit_of(min(tok0 + per, count) - 1) + kTile - 1) / kTile : 0;
-  const int nkv = max(nkv_a, nkv_b);
+  // turns of 64 keys that each tile needs, and tiles of 128 keys
+  const int turns_a = (limit_of(min(tok0 + tokens, count) - 1) + kHalf - 1) / kHalf;
+  const int turns_b = has_b ? (limit_of(min(tok0 + per, count) - 1) + kHalf - 1) / kHalf : 0;
+  const int turns = max(turns_a, turns_b), nkv = (turns + 1) / 2;
 
   if (threadIdx.x == 0) {
     mbar_init(&bar->q_full, 1);
@@ -235,13 +251,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&bar->raw_empty[s], 4);
       mbar_init(&bar->k_full[s], 4);
       mbar_init(&bar->v_full[s], 4);
-      mbar_init(&bar->kv_empty[s], 1);
-      mbar_init(&bar->s_full[s], 1);
-      mbar_init(&bar->p_full[s], 4);
+      mbar_init(&bar->k_empty[s], 2);
+      mbar_init(&bar->v_empty[s], 2);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&bar->s_full[s][i], 1);
+        mbar_init(&bar->p_full[s][i], 4);
+      }
       mbar_init(&bar->o_done[s], 1);
     }
     for (int s = 0; s < kScaleRing; ++s) mbar_init(&bar->scales_full[s], 16);
-    mbar_init(&bar->mma_done, 1);
+    mbar_init(&bar->mma_done, 2);
     fence_mbarrier_init();
   }
   if (warp == 1) {
@@ -256,7 +275,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bar->tmem_base;
-  auto tS = [tmem](int x) -> uint32_t { return tmem + x * 128; };
+  auto tS = [tmem](int x, int i) -> uint32_t { return tmem + x * 128 + (i & 1) * kHalf; };  // of turn i
   auto tO = [tmem](int x) -> uint32_t { return tmem + 256 + x * 128; };
   int* const status = p.status;
 
@@ -289,8 +308,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        // Scales: lane 2y + kv has block y's.  The ring's slot was read for tile j - 4, whose products
-        // were done before the bytes of tile j - 1 were converted.
+        // Scales: lane 2y + kv has block y's.  The ring's slot was read for tile j - 4, before the second
+        // scores of tile j - 3, and those before the keys of tile j - 1 were converted.
         if (j > 0 && !warp_wait(&bar->raw_empty[0], (j - 1) & 1, status, kCacheTimeout)) break;
         const int y = lane >> 1;
         const int tok_y = j * kTile + (y & 7) * kCacheBlock;
@@ -325,62 +344,67 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int loads = (issued + 1 - kv) / 2;
         if (loads > 0) warp_wait(&bar->raw_full[kv], (loads - 1) & 1, status, kCacheTimeout);
       }
-    } else if (warp == 1 && lane == 0) {
-      // ------------------------------------------------------------ MMA issuer
-      const uint32_t idesc_qk = idesc_f16_f32(128, 128, 0);
+    } else if (warp < 3) {
+      // ------------------------------------------------------------ MMA issuer of tile x
+      const uint32_t idesc_qk = idesc_f16_f32(128, kHalf, 0);
       const uint32_t idesc_pv = idesc_f16_f32(128, 128, 1);
-      auto issue_s = [&](int x, int j) {
-        const uint32_t sq = smem_u32(q_tile(smem, x)), sk = smem_u32(k_stage(smem, j & 1));
+      const uint32_t leader = elect_one_sync();
+      const int x = warp - 1, mine = x == 0 ? turns_a : turns_b;
+      auto commit = [&](uint64_t* b) {
+        if (leader) mma_commit(b);
+      };
+      // Descriptors: the address field counts 16 bytes, and no sum of offsets leaves it.
+      const uint64_t dq = smem_desc(smem_u32(smem), 16, 1024, kLayoutSW128);
+      const uint64_t dk = smem_desc(smem_u32(smem + kSmemKV), 16, 1024, kLayoutSW128);
+      const uint64_t dv = smem_desc(smem_u32(smem + kSmemKV + kTileBytes), kChunkBytes, 1024, kLayoutSW128);
+      auto issue_s = [&](int i) {  // keys 64 i .. 64 i + 63
+        const uint64_t a = dq + x * (kTileBytes >> 4), b = dk + (i >> 1 & 1) * (2 * kTileBytes >> 4) + (i & 1) * (kHalf * 128 >> 4);
+        const uint32_t d = tS(x, i);
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-          const uint32_t off = (k >> 2) * kChunkBytes + (k & 3) * 32;
-          mma_bf16_ss(tS(x), smem_desc(sq + off, 16, 1024, kLayoutSW128), smem_desc(sk + off, 16, 1024, kLayoutSW128),
-                      idesc_qk, k > 0 ? 1u : 0u);  // kind::f16: the descriptor says fp16
+          const uint32_t off = ((k >> 2) * kChunkBytes + (k & 3) * 32) >> 4;
+          mma_ss(d, a + off, b + off, idesc_qk, k > 0 ? 1u : 0u, leader);
         }
-        mma_commit(&bar->s_full[x]);
+        commit(&bar->s_full[x][i & 1]);
       };
-      auto issue_pv = [&](int x, int j) {
-        const uint32_t sv = smem_u32(v_stage(smem, j & 1));
+      auto issue_pv = [&](int i) {
+        const uint64_t b = dv + (i >> 1 & 1) * (2 * kTileBytes >> 4) + (i & 1) * (kHalf * 128 >> 4);
+        const uint32_t d = tO(x), a = tS(x, i);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)  // 16 keys: 8 packed columns of P, 2 KB of V
-          mma_ts(tO(x), tS(x) + k * 8, smem_desc(sv + k * 2048, kChunkBytes, 1024, kLayoutSW128), idesc_pv,
-                 (j > 0 || k > 0) ? 1u : 0u);
-        mma_commit(&bar->o_done[x]);
+        for (int k = 0; k < 4; ++k)  // 16 keys: 8 packed columns of P, 2 KB of V
+          mma_ts(d, a + k * 8, b + k * (2048 >> 4), idesc_pv, (i > 0 || k > 0) ? 1u : 0u, leader);
+        commit(&bar->o_done[x]);
       };
-      bool ok = nkv > 0 && mbar_wait(&bar->q_ready, 0, status, kCacheTimeout) &&
-                mbar_wait(&bar->k_full[0], 0, status, kCacheTimeout);
-      if (ok) {
+      int k_seen = -1, v_seen = -1;  // tiles whose keys and values are known to have come
+      auto keys_ready = [&](int tile) {
+        if (tile > k_seen && !warp_wait(&bar->k_full[tile & 1], (tile >> 1) & 1, status, kCacheTimeout)) return false;
+        k_seen = tile;
         tc_fence_after();
-        if (nkv_a > 0) issue_s(0, 0);
-        if (nkv_b > 0) issue_s(1, 0);
+        return true;
+      };
+      auto values_ready = [&](int tile) {
+        if (tile > v_seen && !warp_wait(&bar->v_full[tile & 1], (tile >> 1) & 1, status, kCacheTimeout)) return false;
+        v_seen = tile;
+        return true;
+      };
+      // Both warps give every stage back after it has come, used or not, so that neither is a round ahead.
+      bool ok = nkv > 0 && warp_wait(&bar->q_ready, 0, status, kCacheTimeout) && keys_ready(0);
+      for (int i = 0; ok && i < min(2, mine); ++i) issue_s(i);
+      if (ok) commit(&bar->k_empty[0]);
+      for (int i = 0; ok && i < turns; ++i) {
+        if (i < mine) ok = warp_wait(&bar->p_full[x][i & 1], (i >> 1) & 1, status, kCacheTimeout);
+        if (!ok || !values_ready(i >> 1)) break;
+        tc_fence_after();
+        if (i < mine) issue_pv(i);
+        if ((i & 1) || i == turns - 1) commit(&bar->v_empty[i >> 1 & 1]);
+        if (i + 2 >= turns) continue;
+        if (!keys_ready((i + 2) >> 1)) break;
+        if (i + 2 < mine) issue_s(i + 2);
+        if ((i & 1) || i + 2 == turns - 1) commit(&bar->k_empty[(i + 2) >> 1 & 1]);
       }
-      for (int j = 0; ok && j < nkv; ++j) {
-        const int s = j & 1;
-        bool v_ready = false, k_ready = false;
-        for (int x = 0; x < 2 && ok; ++x) {
-          const int nx = x == 0 ? nkv_a : nkv_b;
-          if (j >= nx) continue;
-          ok = mbar_wait(&bar->p_full[x], j & 1, status, kCacheTimeout);
-          if (ok && !v_ready) ok = mbar_wait(&bar->v_full[s], (j >> 1) & 1, status, kCacheTimeout);
-          if (!ok) break;
-          v_ready = true;
-          tc_fence_after();
-          issue_pv(x, j);
-          if (j + 1 < nx) {
-            if (!k_ready && !mbar_wait(&bar->k_full[(j + 1) & 1], ((j + 1) >> 1) & 1, status, kCacheTimeout)) {
-              ok = false;
-              break;
-            }
-            k_ready = true;
-            tc_fence_after();
-            issue_s(x, j + 1);
-          }
-        }
-        if (ok) mma_commit(&bar->kv_empty[s]);  // every MMA that reads stage s has been issued
-      }
-      // Every MMA that this thread issued completes before TMEM is released.
-      mma_commit(&bar->mma_done);
-      mbar_wait(&bar->mma_done, 0, status, kCacheTimeout);
+      // Every MMA that this warp issued completes before TMEM is released.
+      commit(&bar->mma_done);
+      warp_wait(&bar->mma_done, 0, status, kCacheTimeout);
     }
   } else if (warp >= 12) {
     // -------------------------------------------------------------- converters
@@ -388,10 +412,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int w = warp - 12, r0 = lane & 7, ch0 = lane >> 3;
     for (int j = 0; j < nkv; ++j) {
       const int s = j & 1;
-      if (j >= 2 && !warp_wait(&bar->kv_empty[s], ((j >> 1) - 1) & 1, status, kCacheTimeout)) break;
       bool ok = true;
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
+        if (j >= 2) ok = warp_wait(kv ? &bar->v_empty[s] : &bar->k_empty[s], ((j >> 1) - 1) & 1, status, kCacheTimeout);
         if (ok) ok = warp_wait(&bar->raw_full[kv], j & 1, status, kCacheTimeout);
         if (!ok) break;
         const uint32_t src = smem_u32(raw_buffer(smem, kv));
@@ -431,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------------- softmax + epilogue of tile x
     take_registers<184>();
     const int x = (warp - 4) >> 2, wq = warp & 3, r = wq * 32 + lane;
-    const int tok = tok0 + x * tokens + r / group, my_nkv = x == 0 ? nkv_a : nkv_b;
+    const int tok = tok0 + x * tokens + r / group, my_turns = x == 0 ? turns_a : turns_b;
     const bool valid = r < tokens * group && tok < count;
     const int lim = limit_of(min(tok, count - 1));
     const int min_lim = limit_of(min(tok0 + x * tokens, count - 1));
@@ -473,37 +497,38 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(&bar->q_ready);
     }
     float M = kLowest, l = 0.f;
-    for (int j = 0; j < my_nkv; ++j) {
+    for (int i = 0; i < my_turns; ++i) {
+      const int j = i >> 1;
       if (ok) ok = warp_wait(&bar->scales_full[j % kScaleRing], (j / kScaleRing) & 1, status, kCacheTimeout);
-      if (ok) ok = warp_wait(&bar->s_full[x], j & 1, status, kCacheTimeout);
+      if (ok) ok = warp_wait(&bar->s_full[x][i & 1], (i >> 1) & 1, status, kCacheTimeout);
       if (!ok) break;
       tc_fence_after();
-      float sv[128];
+      float sv[kHalf];
       {
-        uint32_t raw[4][32];
+        uint32_t raw[2][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32_nowait(tS(x) + lane_off + c * 32, raw[c]);
+        for (int c = 0; c < 2; ++c) tmem_ld32_nowait(tS(x, i) + lane_off + c * 32, raw[c]);
         tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) sv[c * 32 + i] = __uint_as_float(raw[c][i]);
+          for (int e = 0; e < 32; ++e) sv[c * 32 + e] = __uint_as_float(raw[c][e]);
       }
-      const int rel = lim - j * kTile;  // columns below it are seen
-      const float4* sc = reinterpret_cast<const float4*>(scale_ring + (j % kScaleRing) * 16);
+      const int rel = lim - i * kHalf;  // columns below it are seen
+      const float4* sc = reinterpret_cast<const float4*>(scale_ring + (j % kScaleRing) * 16 + (i & 1) * 8);
       float alpha = 1.f;
       bool rescale = false;
-      uint32_t pk[64];
+      uint32_t pk[32];
       // Tiles that some row sees only in part are masked; the others do without those instructions.
       auto probabilities = [&](auto masked) {
         constexpr bool kMasked = decltype(masked)::value;
         if (kMasked) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c) sv[c] = c >= rel ? -INFINITY : sv[c];
+          for (int c = 0; c < kHalf; ++c) sv[c] = c >= rel ? -INFINITY : sv[c];
         }
-        float mult[8], ev[8], inv[8];  // of the blocks: the scores' factor, log2 of the values' scale, its inverse
+        float mult[4], ev[4], inv[4];  // of the blocks: the scores' factor, log2 of the values' scale, its inverse
 #pragma unroll
-        for (int y = 0; y < 8; y += 2) {
+        for (int y = 0; y < 4; y += 2) {
           const float4 two = sc[y / 2];
           mult[y] = factor * two.x, mult[y + 1] = factor * two.z;
           // NaN stays NaN
@@ -514,7 +539,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         float mx = kLowest;
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
+        for (int y = 0; y < 4; ++y) {
           const float* v = sv + y * 16;
           const float t0 = max3(v[0], v[1], v[2]), t1 = max3(v[3], v[4], v[5]), t2 = max3(v[6], v[7], v[8]);
           const float t3 = max3(v[9], v[10], v[11]), t4 = max3(v[12], v[13], v[14]);
@@ -522,14 +547,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (mx > M + kRescaleThreshold) {
           alpha = fast_exp2(M - mx);
-          rescale = j > 0;
+          rescale = i > 0;
           M = mx;
         }
         l *= alpha;
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
+        for (int y = 0; y < 4; ++y) {
           const uint64_t m2 = pair_of(mult[y], mult[y]), a2 = pair_of(ev[y] - M, ev[y] - M);
-          uint64_t sum = pair_of(0.f, 0.f);
+          float sA = 0.f, sB = 0.f;
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             const int col = y * 16 + 2 * c;
@@ -540,48 +565,44 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (col >= rel) a = 0.f;
               if (col + 1 >= rel) d = 0.f;
             }
-            sum = add_pair(sum, pair_of(a, d));
+            sA += a; sB += d;
             pk[y * 8 + c] = half2_bits(a, d);
           }
-          float s0, s1;
-          split_pair(sum, s0, s1);
-          const float both = s0 + s1;
+          const float both = sA + sB;
           if (!kMasked || both != 0.f) l = fmaf(both, inv[y], l);  // a block that is not seen adds nothing
         }
       };
-      if ((j + 1) * kTile > min_lim) probabilities(std::true_type{});
+      if ((i + 1) * kHalf > min_lim) probabilities(std::true_type{});
       else probabilities(std::false_type{});
-      // P_x(j) overwrites the columns that PV_x(j-1) reads, and a rescale touches O_x: both wait for it.
-      if (j > 0) {
-        ok = warp_wait(&bar->o_done[x], (j - 1) & 1, status, kCacheTimeout);
+      if (__any_sync(0xffffffff, rescale)) {  // O is touched: its last product has to be done
+        ok = warp_wait(&bar->o_done[x], (i - 1) & 1, status, kCacheTimeout);
         if (!ok) break;
         tc_fence_after();
-        if (__any_sync(0xffffffff, rescale)) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float ov[32];
-            tmem_ld32(tO(x) + lane_off + c * 32, ov);
+        for (int c = 0; c < 4; ++c) {
+          float ov[32];
+          tmem_ld32(tO(x) + lane_off + c * 32, ov);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) ov[i] *= alpha;
-            tmem_st32(tO(x) + lane_off + c * 32, ov);
-          }
+          for (int e = 0; e < 32; ++e) ov[e] *= alpha;
+          tmem_st32(tO(x) + lane_off + c * 32, ov);
         }
       }
-      tmem_st32_u(tS(x) + lane_off, pk);
-      tmem_st32_u(tS(x) + lane_off + 32, pk + 32);
+      tmem_st32_u(tS(x, i) + lane_off, pk);  // over scores that have been loaded
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bar->p_full[x]);
+      if (lane == 0) mbar_arrive(&bar->p_full[x][i & 1]);
     }
-    if (ok && my_nkv > 0) ok = warp_wait(&bar->o_done[x], (my_nkv - 1) & 1, status, kCacheTimeout);
+    // The last S came after all products but two: wait for either, since a parity tells only neighbours apart.
+    if (ok && my_turns > 1) ok = warp_wait(&bar->o_done[x], (my_turns - 2) & 1, status, kCacheTimeout);
+    if (ok && my_turns > 0) ok = warp_wait(&bar->o_done[x], (my_turns - 1) & 1, status, kCacheTimeout);
     tc_fence_after();
     const float inv_l = l > 0.f || l != l ? 1.f / l : 0.f;
     uint4* dst = reinterpret_cast<uint4*>(p.out) + ((int64_t)(first_row + tok) * p.H + kvh * group + r % group) * (kCacheDim / 8);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       float ov[32];
-      if (ok && my_nkv > 0) {
+      if (ok && my_turns > 0) {
         tmem_ld32(tO(x) + lane_off + c * 32, ov);
       } else {
 #pragma unroll
