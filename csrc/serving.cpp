@@ -352,11 +352,17 @@ at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at
   auto stream = at::cuda::getCurrentCUDAStream();
   const bool bf16 = q.scalar_type() == at::kBFloat16;
   // (q strides of zero, a broadcast, are not for a tensor map)
-  const int64_t most_rows = (max_new < 1 ? q.size(0) : std::min(max_new, q.size(0))) * p.group;
-  const int64_t tiles = (q.size(0) * p.group / 256 + n) * KV;
   const bool can = p.group <= 64 && p.scale_log2 > 0.f && q.stride(0) > 0 && q.stride(1) > 0;
   SERVING_CHECK(kernel != 2 || can, "the prompt kernel cannot take these arguments");
-  if (kernel == 2 || (kernel == 0 && can && most_rows >= 64 && tiles >= 74)) {
+  // Both kernels' times grow with the keys alike.  The one that splits them takes 4.2 ns for 16 rows and 64
+  // keys on the whole GPU, the prompt kernel 1.05 us for the 256 rows of each of 148 blocks.  Measured on both
+  // sides of the line (split / prompt): 4096 keys, 4 key/value heads, 16 heads, one sequence, 128 new tokens
+  // 60 / 83 us, 256 88 / 84; 16 sequences, 8 new 61 / 65, 16 90 / 65; 64 sequences, 4 new 100 / 135, 8 165 / 136;
+  // 16 and 16 heads, 16 sequences, 16 new 100 / 134, 32 166 / 134.
+  const int64_t row_tiles = KV * std::max<int64_t>(n, (q.size(0) * p.group + 15) / 16);
+  const int64_t per = p.group <= 64 ? 2 * (128 / p.group) : 1;
+  const int64_t blocks = KV * std::max<int64_t>(n, (q.size(0) + per - 1) / per);
+  if (kernel == 2 || (kernel == 0 && can && row_tiles >= 250 * ((blocks + 147) / 148))) {
     const CUtensorMap map_q = queries_map(q, p.group), map_pages = pages_map(pages, kPromptKeys);
     for (int64_t base = 0; base < n; base += kAttentionSeqs) {
       p.n = (int)std::min<int64_t>(kAttentionSeqs, n - base);
@@ -379,8 +385,8 @@ at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at
     p.prefix = prefix_lens.has_value() ? prefix_lens->data_ptr<int>() + base : nullptr;
     p.last_batch = base + p.n == n;
     // no more blocks than units: at most this many
-    const int64_t row_tiles = std::min<int64_t>(q.size(0), p.n) + q.size(0) * p.group / kAttentionRows + 1;
-    const int64_t most = row_tiles * KV * (((int64_t)p.width * p.page + kAttentionKeys - 1) / kAttentionKeys + 1 + kAttentionEnds);
+    const int64_t segments = std::min<int64_t>(q.size(0), p.n) + q.size(0) * p.group / kAttentionRows + 1;
+    const int64_t most = segments * KV * (((int64_t)p.width * p.page + kAttentionKeys - 1) / kAttentionKeys + 1 + kAttentionEnds);
     const int grid = (int)std::min<int64_t>(kAttentionBlocks, std::max<int64_t>(most, 1));
     at::Tensor work = at::empty({grid * (int64_t)(2 * kAttentionRows * (kCacheDim + 2))}, q.options().dtype(at::kFloat));
     p.parts = work.data_ptr<float>();

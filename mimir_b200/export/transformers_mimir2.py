@@ -22,6 +22,9 @@ from z_H with no injection and H follows L directly).  Attention is prefix-LM: t
 For generation every stack invocation keeps its own KV cache (virtual layer ``invocation *
 layers + layer``) and the prompt is the prefix.
 
+Serving may keep the keys and values in 8 bits instead: :meth:`Mimir2Model.forward_paged` runs packed
+sequences over the paged cache of :mod:`mimir_b200.serving.paged`.
+
 Mixtures of experts or stacks, residual branches and recurrent memories are not implemented by
 this model (the export's own :class:`mimir_b200.export.hf.Mimir2ForCausalLM` runs those).
 """
@@ -116,7 +119,15 @@ class Mimir2Attention(nn.Module):
         self.v_proj = nn.Linear(d, kv * hd, bias=False)
         self.o_proj = nn.Linear(h * hd, d, bias=False)
 
+    def _paged(self, x, batch, layer_idx: int):
+        """Packed rows ``x [tokens, d]`` over the 8-bit paged cache, which rotates q and k itself."""
+        gate, q, k, v = (proj(x).unflatten(-1, (-1, self.head_dim))
+                         for proj in (self.gate_proj, self.q_proj, self.k_proj, self.v_proj))
+        return self.o_proj((torch.sigmoid(gate) * batch.attend(layer_idx, q, k, v)).flatten(-2))
+
     def forward(self, x, rope, mask, cache: Optional[DynamicCache], layer_idx: int):
+        if x.ndim == 2:
+            return self._paged(x, cache, layer_idx)
         b, s, _ = x.shape
         shape = (b, s, -1, self.head_dim)
         gate = self.gate_proj(x).view(shape)
@@ -244,6 +255,31 @@ class Mimir2Model(Mimir2PreTrainedModel):
             x = self.ngram(x, input_ids, position_ids, history)
         rope = self.rope(position_ids)
         mask = self._mask(b, s, past, prefix_lengths if cfg.prefix_lm else None, x.device, x.dtype, key_valid)
+        return self._recur(x, rope, mask, past_key_values)
+
+    def forward_paged(self, tokens, batch):
+        """Hidden states ``[tokens, hidden]`` of the packed new ``tokens`` of a
+        :class:`mimir_b200.serving.paged.Batch`, whose cache takes their keys and values."""
+        x = self.embed_tokens(tokens) * self.config.embedding_scale
+        if self.config.ngram_orders:
+            x = self._paged_ngram(x, tokens, batch)
+        return self._recur(x, None, None, batch)
+
+    def _paged_ngram(self, x, tokens, batch):
+        history = getattr(batch, "ngram_history", None)
+        if history is None:  # whole prompts: no n-gram reaches across their first positions
+            return self.ngram(x[None], tokens[None], batch.positions()[None].long())[0]
+        # one token a sequence: it and the ones before it, from the slots' histories
+        tail = max(self.config.ngram_orders) - 1
+        at = torch.tensor(batch.ngram_lens, device=x.device)[:, None] - 1 + torch.arange(-tail, 1, device=x.device)
+        slots = torch.tensor(batch.slots, device=x.device)[:, None]
+        ids = history[slots, at.clamp_min(0)].long()
+        positions = torch.where(at < 0, 1000 * at - 1000, at)  # no neighbours before the first token
+        wide = torch.cat((x.new_zeros(x.shape[0], tail, x.shape[1]), x[:, None]), dim=1)
+        return self.ngram(wide, ids, positions)[:, -1]
+
+    def _recur(self, x, rope, mask, past_key_values):
+        cfg = self.config
         layers = cfg.num_layers_per_stack
         looped = cfg.recurrence_mode == "looped"
         z_h, z_l = x, self.z_L_init.to(x.dtype)

@@ -15,8 +15,8 @@ A batch of new tokens is ``seqs`` (int32, the slot of each sequence, each at mos
 (int32, one more entry): sequence ``i`` has the rows ``cu_new[i]:cu_new[i + 1]``, and they are the last
 tokens of its slot: :func:`cache_reserve` has counted them in ``seq_lens`` already.
 
-On CUDA every function is a kernel of ``csrc/kv_cache.cu`` or ``csrc/cache_attention.cu`` on the
-current stream and does not synchronise.  Arguments of a wrong type
+On CUDA every function runs kernels of ``csrc/kv_cache.cu``, ``csrc/cache_attention.cu`` (few rows) and
+``csrc/cache_prompt.cu`` (many) on the current stream and does not synchronise.  Arguments of a wrong type
 or shape raise ``ValueError``; slots, pages and lengths that lie in device memory are checked by the
 kernels: a bad one is skipped and reported by :func:`mimir_b200.ops._ext.check_kernel_status`.  On the
 CPU the PyTorch formulations below run, which also take other head dimensions and float32 rows.
@@ -150,8 +150,8 @@ def cache_attention(q, pages, scales, page_table, seq_lens, seqs, cu_new, prefix
     :func:`mimir_b200.ops.prefixlm_attention`).  A token that sees nothing, and rows beyond
     ``cu_new[-1]``, give zeros.  ``softmax_scale`` is ``head_dim ** -0.5`` by default.
 
-    ``max_new`` (the most new tokens of one sequence, if known on the host) chooses between kernels
-    and changes no result beyond rounding.
+    ``max_new`` (the most new tokens of one sequence, if known on the host) lets few rows take a narrower
+    kernel; it changes no result beyond rounding.
     """
     if softmax_scale is None:
         softmax_scale = q.shape[-1] ** -0.5

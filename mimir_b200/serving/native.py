@@ -24,8 +24,14 @@ first token) and decodes them together, which gives each greedy request its own 
 continuation and each sampled request independent samples.  Seeded or streamed requests run one
 at a time.
 
+``--kv-cache fp8`` decodes over the 8-bit paged cache instead (:mod:`mimir_b200.serving.paged`; on CUDA a
+bfloat16 or float16 model with heads of 128): half the memory of a 16-bit cache and no padding, so that
+requests of any decoding rule and any seed share a batch, and the further fields ``n`` (completions that share
+the prompt's pages), ``presence_penalty``, ``frequency_penalty``, ``repetition_penalty``, ``logit_bias`` and
+``allowed_token_ids``.
+
 Usage: ``python -m mimir_b200.serving.native MODEL_DIR [--port 8000] [--device cuda:0]
-[--max-batch 8] [--batch-wait-ms 5]``.
+[--max-batch 8] [--batch-wait-ms 5] [--kv-cache model|fp8]``.
 """
 from __future__ import annotations
 
@@ -56,10 +62,12 @@ class Engine:
     finish_reason)``."""
 
     def __init__(self, model_dir, device: str = "cpu", dtype: Optional[torch.dtype] = None, name: Optional[str] = None,
-                 max_batch: int = 8, batch_wait_ms: float = 5.0):
+                 max_batch: int = 8, batch_wait_ms: float = 5.0, kv_cache: str = "model"):
         from transformers import AutoModelForCausalLM, AutoTokenizer
 
         from mimir_b200.export.transformers_mimir2 import register
+        if kv_cache not in ("model", "fp8"):
+            raise ValueError(f"kv_cache must be model or fp8, not {kv_cache}")
         register()
         self.name = name or Path(model_dir).name
         self.device = torch.device(device)
@@ -72,6 +80,10 @@ class Engine:
         self.batch_wait = max(0.0, float(batch_wait_ms)) / 1000.0
         self.pad_id = (self.tokenizer.pad_token_id if self.tokenizer.pad_token_id is not None
                        else self.tokenizer.eos_token_id if self.tokenizer.eos_token_id is not None else 0)
+        self.paged = None
+        if kv_cache == "fp8":
+            from mimir_b200.serving.paged import PagedDecoder
+            self.paged = PagedDecoder(self.model, slots=2 * self.max_batch)
         self._queue: list[_Pending] = []
         self._ready = threading.Condition()
         if self.max_batch > 1:
@@ -113,16 +125,39 @@ class Engine:
         return text, len(ids), len(new), finish
 
     def batchable(self, body: dict) -> bool:
-        return self.max_batch > 1 and body.get("seed") is None
+        return self.max_batch > 1 and (self.paged is not None or body.get("seed") is None)
 
-    @staticmethod
-    def _sampling(body: dict) -> tuple:
-        """Requests share a batch only with the same decoding rule (greedy, or one temperature/top-p)."""
+    def _sampling(self, body: dict) -> tuple:
+        """Requests share a batch only with the same decoding rule (greedy, or one temperature/top-p); over the
+        paged cache every row has its own."""
+        if self.paged is not None:
+            return ()
         temperature = float(body.get("temperature") or 0.0)
         return (temperature, float(body.get("top_p") or 1.0)) if temperature > 0 else (0.0, 1.0)
 
+    def _request(self, ids: list[int], body: dict):
+        from mimir_b200.serving.paged import Request
+        request = Request(ids, max_tokens=self._max_tokens(body), temperature=float(body.get("temperature") or 0.0),
+                          top_p=float(body.get("top_p") or 1.0), n=int(body.get("n") or 1),
+                          seed=None if body.get("seed") is None else int(body["seed"]),
+                          presence_penalty=float(body.get("presence_penalty") or 0.0),
+                          frequency_penalty=float(body.get("frequency_penalty") or 0.0),
+                          repetition_penalty=float(body.get("repetition_penalty") or 1.0),
+                          logit_bias={int(k): float(v) for k, v in (body.get("logit_bias") or {}).items()},
+                          allowed_token_ids=body.get("allowed_token_ids"))
+        request.check(self.model.config.vocab_size, self.model.config.max_position_embeddings)
+        return request
+
+    def complete_all(self, ids: list[int], body: dict) -> list[tuple[str, int, int, str]]:
+        """:meth:`complete` of each of the request's ``n`` completions (one without the paged cache)."""
+        result = self.complete(ids, body)
+        return result if isinstance(result, list) else [result]
+
     @torch.no_grad()
-    def complete(self, ids: list[int], body: dict) -> tuple[str, int, int, str]:
+    def complete(self, ids: list[int], body: dict):
+        """One result, or a list of them where a request over the paged cache asks for ``n > 1``."""
+        if self.paged is not None:
+            self._request(ids, body)  # a bad request fails by itself, not with the batch it would be in
         if self.batchable(body):
             item = _Pending(ids, body)
             with self._ready:
@@ -132,6 +167,8 @@ class Engine:
             if item.error is not None:
                 raise item.error
             return item.result
+        if self.paged is not None:
+            return self._generate_batch([_Pending(ids, body)])[0]
         temperature = float(body.get("temperature") or 0.0)
         gen = self._gen_args(self._max_tokens(body)) | dict(do_sample=temperature > 0)
         if temperature > 0:
@@ -146,6 +183,9 @@ class Engine:
     def stream(self, ids: list[int], body: dict):
         """Yield decoded text pieces as they are generated, then ``(None, result)`` where result
         is what :meth:`complete` returns (stop strings cut the text and end the stream early)."""
+        if self.paged is not None:
+            yield from self._stream_paged(ids, body)
+            return
         from transformers import TextIteratorStreamer
         temperature = float(body.get("temperature") or 0.0)
         gen = self._gen_args(self._max_tokens(body)) | dict(do_sample=temperature > 0)
@@ -186,6 +226,31 @@ class Engine:
         result = self._finish(ids, holder["out"][0, len(ids):].tolist(), body)
         yield None, (sent, result[1], result[2], "stop" if stopped else result[3])
 
+    def _stream_paged(self, ids: list[int], body: dict):
+        request = self._request(ids, body | {"n": 1})
+        stops = body.get("stop") or []
+        stops = [stops] if isinstance(stops, str) else [x for x in stops if x]
+        new, sent, stopped = [], "", False
+        with self.lock:
+            for _, _, token in self.paged.run([request], self.tokenizer.eos_token_id):
+                new.append(token)
+                text = self.tokenizer.decode(new, skip_special_tokens=True)
+                cut = min((text.find(x) for x in stops if x in text), default=-1)
+                if cut >= 0:
+                    text, stopped = text[:cut], True
+                elif text.endswith("\ufffd"):
+                    continue  # part of a character
+                if len(text) > len(sent):
+                    yield text[len(sent):], None
+                    sent = text
+                if stopped:
+                    break
+        text, n_in, n_out, finish = self._finish(ids, new, body)
+        if not stopped and len(text) > len(sent):
+            yield text[len(sent):], None
+            sent = text
+        yield None, (sent, n_in, n_out, "stop" if stopped else finish)
+
     # ------------------------------------------------------------------ batched greedy decoding
     def _serve_batches(self) -> None:
         while True:
@@ -215,6 +280,11 @@ class Engine:
 
     @torch.no_grad()
     def _generate_batch(self, batch: list[_Pending]) -> list:
+        if self.paged is not None:
+            with self.lock:
+                out = self.paged.generate([self._request(item.ids, item.body) for item in batch], self.tokenizer.eos_token_id)
+            results = [[self._finish(item.ids, new, item.body) for new in each] for item, each in zip(batch, out)]
+            return [r if len(r) > 1 else r[0] for r in results]
         width = max(len(item.ids) for item in batch)
         x = torch.full((len(batch), width), self.pad_id, dtype=torch.long)
         mask = torch.zeros_like(x)
@@ -263,18 +333,21 @@ def _handler(engine: Engine):
                 ids = engine.prompt_ids(body, chat)
                 if body.get("stream"):
                     return self._stream(engine.stream(ids, body), chat)
-                text, n_in, n_out, finish = engine.complete(ids, body)
+                results = engine.complete_all(ids, body)
             except (KeyError, ValueError, TypeError) as exc:
                 return self._send(400, {"error": {"message": str(exc)}})
+            n_in, n_out = results[0][1], sum(r[2] for r in results)
             usage = {"prompt_tokens": n_in, "completion_tokens": n_out, "total_tokens": n_in + n_out}
             base = {"id": f"cmpl-{uuid.uuid4().hex}", "created": int(time.time()), "model": engine.name,
                     "usage": usage}
             if chat:
                 self._send(200, base | {"object": "chat.completion", "choices": [
-                    {"index": 0, "message": {"role": "assistant", "content": text}, "finish_reason": finish}]})
+                    {"index": i, "message": {"role": "assistant", "content": text}, "finish_reason": finish}
+                    for i, (text, _, _, finish) in enumerate(results)]})
             else:
                 self._send(200, base | {"object": "text_completion", "choices": [
-                    {"index": 0, "text": text, "finish_reason": finish}]})
+                    {"index": i, "text": text, "finish_reason": finish}
+                    for i, (text, _, _, finish) in enumerate(results)]})
         def _stream(self, pieces, chat: bool) -> None:
             cid, created = f"cmpl-{uuid.uuid4().hex}", int(time.time())
             kind = "chat.completion.chunk" if chat else "text_completion"
@@ -323,9 +396,11 @@ def main(argv=None) -> None:
     ap.add_argument("--dtype", choices=["float32", "bfloat16"], default=None)
     ap.add_argument("--max-batch", type=int, default=8, help="greedy requests decoded together (1: one at a time)")
     ap.add_argument("--batch-wait-ms", type=float, default=5.0, help="how long a batch waits for more requests")
+    ap.add_argument("--kv-cache", choices=["model", "fp8"], default="model",
+                    help="fp8: decode over the 8-bit paged cache (needs --dtype bfloat16 on CUDA)")
     args = ap.parse_args(argv)
     engine = Engine(args.model, args.device, getattr(torch, args.dtype) if args.dtype else None,
-                    max_batch=args.max_batch, batch_wait_ms=args.batch_wait_ms)
+                    max_batch=args.max_batch, batch_wait_ms=args.batch_wait_ms, kv_cache=args.kv_cache)
     server = make_server(engine, args.host, args.port)
     print(f"serving {engine.name} on http://{args.host}:{args.port}/v1", flush=True)
     server.serve_forever()

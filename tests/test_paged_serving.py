@@ -1,0 +1,246 @@
+"""Serving over the 8-bit paged cache (``mimir_b200.serving.paged``, ``Engine(kv_cache="fp8")``): the same
+hidden states as the model's own cache up to the 8 bits, completions that do not depend on what
+else is in the batch, forks, growth of the pool, request fields and refusals.  CPU: the PyTorch
+formulations; ``-m gpu``: the kernels."""
+import json
+import threading
+import urllib.request
+
+import pytest
+import torch
+
+pytest.importorskip("transformers")
+
+from mimir_b200.serving.paged import PagedDecoder, Request  # noqa: E402
+
+VARIANTS = [dict(), dict(gates_enabled=True), dict(ngram_orders=[2, 3], ngram_buckets=97, ngram_heads=2,
+                                                   ngram_contextual_gate=True),
+            dict(recurrence_mode="looped")]
+
+
+def _model(tmp_path, extra=None, device="cpu", dtype=torch.float32):
+    from transformers import AutoModelForCausalLM
+    from test_transformers_model import _export
+    from mimir_b200.export.transformers_mimir2 import register
+    register()
+    _export(tmp_path, extra or {})
+    return AutoModelForCausalLM.from_pretrained(tmp_path, dtype=dtype).to(device).eval()
+
+
+class PlainBatch:
+    """A :class:`mimir_b200.serving.paged.Batch` whose keys and values keep their type: the formula."""
+
+    def __init__(self, batch, kept):
+        self.batch, self.kept = batch, kept  # kept[layer, slot] -> (keys, values)
+        self.slots = batch.slots
+
+    def positions(self):
+        return self.batch.positions()
+
+    def attend(self, layer, q, k, v):
+        b, out = self.batch, torch.zeros_like(q)
+        pos = b.positions()
+        cos, sin = b.cache.cos[pos][:, None], b.cache.sin[pos][:, None]
+        half = q.shape[-1] // 2
+
+        def turn(x):
+            return x.float() * cos + torch.cat((-x[..., half:], x[..., :half]), -1).float() * sin
+
+        q, k = turn(q), turn(k)
+        start = 0
+        for slot, count in zip(b.slots, b.counts):
+            rows = slice(start, start + count)
+            old = self.kept.get((layer, slot))
+            keys, values = k[rows], v[rows].float()
+            if old is not None:
+                keys, values = torch.cat((old[0], keys)), torch.cat((old[1], values))
+            self.kept[layer, slot] = keys, values
+            group = q.shape[1] // keys.shape[1]
+            s = torch.einsum("thd,jhd->htj", q[rows], keys.repeat_interleave(group, 1)) * q.shape[-1] ** -0.5
+            if b.prefix_lens is None:
+                seen = torch.arange(keys.shape[0], device=s.device) <= pos[rows][:, None]
+                s = s.masked_fill(~seen, -torch.inf)
+            out[rows] = torch.einsum("htj,jhd->thd", s.softmax(-1), values.repeat_interleave(group, 1)).to(out.dtype)
+            start += count
+        return out
+
+
+def _teacher_forced(model, prompts, tails, plain=False):
+    """Logits of the packed path for prompts and then given tokens, one at a time."""
+    dec = PagedDecoder(model, page_size=16, pages=3, slots=4)
+    cache, dev, slots = dec.cache, dec.device, list(range(len(prompts)))
+    kept = {}
+
+    def forward(ids, batch):
+        return model.model.forward_paged(ids.to(dev), batch)
+
+    cache.reserve(slots, [len(p) for p in prompts])
+    batch = cache.batch(slots, [len(p) for p in prompts], prompts=True)
+    hidden = forward(torch.tensor(sum(prompts, [])), PlainBatch(batch, kept) if plain else batch)
+    out = [[x] for x in model.lm_head(hidden[batch.last_rows])]
+    for s, p in zip(slots, prompts):
+        dec.history[s, :len(p)] = torch.tensor(p, dtype=torch.int32)
+    for t in range(len(tails[0])):
+        ids = torch.tensor([tail[t] for tail in tails])
+        lens = [len(p) + t + 1 for p in prompts]
+        dec.history[torch.tensor(slots), torch.tensor(lens) - 1] = ids.to(dev, torch.int32)
+        cache.reserve(slots, [1] * len(slots))
+        batch = cache.batch(slots, [1] * len(slots))
+        batch = PlainBatch(batch, kept) if plain else batch
+        batch.ngram_history, batch.ngram_lens = dec.history, lens
+        for row, x in zip(out, model.lm_head(forward(ids, batch))):
+            row.append(x)
+    return torch.stack([torch.stack(rows) for rows in out]).float()
+
+
+def _both(model, vocab=96):
+    """(prompts, tails, the model's own logits where they are predicted)."""
+    gen = torch.Generator().manual_seed(3)
+    prompts = [torch.randint(0, vocab, (n,), generator=gen).tolist() for n in (5, 1, 23)]
+    tails = [torch.randint(0, vocab, (6,), generator=gen).tolist() for _ in prompts]
+    full = [model(torch.tensor([p + t]).to(model.device), prefix_lengths=torch.tensor([len(p)])).logits[0, len(p) - 1:]
+            for p, t in zip(prompts, tails)]
+    return prompts, tails, torch.stack(full).float()
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("extra", VARIANTS, ids=["plain", "gates", "ngram", "looped"])
+def test_packed_forward_is_the_model(tmp_path, extra):
+    """With keys and values as they are, the packed path gives the model's logits (float32: 12 layer calls of
+    sums of at most 256 products, each rounded to 2^-24); with the 8 bits it comes near."""
+    model = _model(tmp_path, extra)
+    prompts, tails, full = _both(model)
+    torch.testing.assert_close(_teacher_forced(model, prompts, tails, plain=True), full, atol=2e-4, rtol=2e-4)
+    got = _teacher_forced(model, prompts, tails)
+    assert 0 < (got - full).norm() < 0.5 * full.norm()
+
+
+def test_completions_do_not_depend_on_the_batch(tmp_path):
+    dec = PagedDecoder(_model(tmp_path), page_size=16, pages=1, slots=2)  # the pool and the slots have to grow
+    reqs = [Request([3, 1, 4, 1, 5], max_tokens=7), Request([9] * 30, max_tokens=4, n=3),
+            Request([2, 6], max_tokens=9, temperature=0.9, top_p=0.8, seed=5, n=2),
+            Request([5, 3, 5], max_tokens=6, presence_penalty=1.5, frequency_penalty=0.5, repetition_penalty=1.3)]
+    together = dec.generate(reqs)
+    assert [len(x) for x in together] == [1, 3, 2, 1]
+    assert [len(x[0]) for x in together] == [7, 4, 9, 6]
+    assert together[1][0] == together[1][1] == together[1][2]  # greedy forks agree
+    for r, want in zip(reqs, together):
+        assert dec.generate([r])[0] == want
+    assert int(dec.cache.ref_counts.sum()) == 0 and int(dec.cache.seq_lens.sum()) == 0  # all given back
+
+
+def test_request_fields(tmp_path):
+    dec = PagedDecoder(_model(tmp_path), slots=8)
+    prompt = [7, 7, 8]
+    plain = dec.generate([Request(prompt, max_tokens=8)])[0][0]
+    only = dec.generate([Request(prompt, max_tokens=8, allowed_token_ids=[11, 95])])[0][0]
+    assert set(only) <= {11, 95}
+    assert dec.generate([Request(prompt, max_tokens=3, logit_bias={42: 1000.0})])[0][0] == [42] * 3
+    banned = dec.generate([Request(prompt, max_tokens=1, logit_bias={plain[0]: -1000.0})])[0][0]
+    assert banned != plain[:1]
+    # a presence penalty beyond all differences forbids repetition
+    once = dec.generate([Request(prompt, max_tokens=20, presence_penalty=1000.0)])[0][0]
+    assert len(set(once)) == 20
+    assert dec.generate([Request(prompt, max_tokens=20)], eos=plain[2])[0][0] == plain[:plain.index(plain[2]) + 1]
+    for bad in (Request([], 4), Request([96], 4), Request([1] * 64, 4), Request([1], 4, n=0), Request([1], 0),
+                Request([1], 4, logit_bias={96: 1.0}), Request([1], 4, allowed_token_ids=[])):
+        with pytest.raises(ValueError):
+            dec.generate([bad])
+    assert dec.generate([Request(prompt, max_tokens=8)])[0][0] == plain
+    assert len(dec.generate([Request([1] * 60, max_tokens=50)])[0][0]) == 4  # 64 positions
+
+
+def _post(url, body):
+    req = urllib.request.Request(url, data=json.dumps(body).encode(), headers={"Content-Type": "application/json"})
+    try:
+        with urllib.request.urlopen(req, timeout=60) as r:
+            return r.status, r.read()
+    except urllib.error.HTTPError as exc:
+        return exc.code, exc.read()
+
+
+def _serve(tmp_path, device, **kw):
+    from test_native_serving import _tokenizer
+    from mimir_b200.serving.native import Engine, make_server
+    _tokenizer(tmp_path)
+    engine = Engine(tmp_path, device, name="tiny", max_batch=4, batch_wait_ms=100, kv_cache="fp8", **kw)
+    server = make_server(engine, "127.0.0.1", 0)
+    threading.Thread(target=server.serve_forever, daemon=True).start()
+    return engine, server, f"http://127.0.0.1:{server.server_address[1]}/v1/completions"
+
+
+def _check_server(engine, server, url):
+    try:
+        bodies = [{"prompt": "w1 w2 w3", "max_tokens": 5}, {"prompt": "w4", "max_tokens": 4, "n": 3},
+                  {"prompt": "w5 w6", "max_tokens": 6, "temperature": 0.7, "seed": 3},
+                  {"prompt": "w7 w8", "max_tokens": 5, "logit_bias": {"10": 500}, "presence_penalty": 0.5}]
+        alone = [json.loads(_post(url, b)[1]) for b in bodies]
+        got = [None] * len(bodies)
+
+        def ask(i):
+            got[i] = json.loads(_post(url, bodies[i])[1])
+
+        threads = [threading.Thread(target=ask, args=(i,)) for i in range(len(bodies))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(timeout=120)
+        for body, a, b in zip(bodies, alone, got):
+            assert a["choices"] == b["choices"] and a["usage"] == b["usage"]
+            assert len(a["choices"]) == body.get("n", 1) and [c["index"] for c in a["choices"]] == list(range(body.get("n", 1)))
+        assert alone[1]["usage"]["completion_tokens"] <= 12 and alone[3]["choices"][0]["text"].split()[0] == "w10"
+        status, raw = _post(url, bodies[0] | {"stream": True})
+        lines = [x[6:] for x in raw.decode().splitlines() if x.startswith("data: ")]
+        assert status == 200 and lines[-1] == "[DONE]"
+        assert "".join(json.loads(x)["choices"][0]["text"] for x in lines[:-1]) == alone[0]["choices"][0]["text"]
+        assert _post(url, {"prompt": "w1", "n": 0 - 1})[0] == 400
+        assert _post(url, {"prompt": "w1", "repetition_penalty": -2})[0] == 400
+    finally:
+        server.shutdown()
+        server.server_close()
+
+
+def test_native_server_over_the_paged_cache(tmp_path):
+    from test_transformers_model import _export
+    _export(tmp_path, {})
+    _check_server(*_serve(tmp_path, "cpu"))
+    from mimir_b200.serving.native import Engine
+    with pytest.raises(ValueError, match="model or fp8"):
+        Engine(tmp_path, "cpu", kv_cache="int4")
+
+
+# ---------------------------------------------------------------------------------- GPU
+GPU = dict(hidden_size=256, num_heads=2, num_key_value_heads=1, max_seq_len=512)  # heads of 128
+
+
+@pytest.mark.gpu
+@torch.no_grad()
+@pytest.mark.parametrize("extra", VARIANTS, ids=["plain", "gates", "ngram", "looped"])
+def test_paged_forward_on_the_gpu(tmp_path, extra, monkeypatch):
+    """The kernels are as near to the model as their PyTorch formulations on the same GPU (which round to the
+    same 8 bits, and to bfloat16 in the same places)."""
+    model = _model(tmp_path, GPU | extra, "cuda", torch.bfloat16)
+    prompts, tails, full = _both(model)
+    got = _teacher_forced(model, prompts, tails)
+    monkeypatch.setenv("MIMIR_DISABLE_KERNELS", "1")
+    formula = _teacher_forced(model, prompts, tails)
+    assert (got - full).norm() <= 1.5 * (formula - full).norm()
+
+
+@pytest.mark.gpu
+def test_server_on_the_gpu(tmp_path):
+    from mimir_b200.ops._ext import check_kernel_status, launch_count
+    from test_transformers_model import _export
+    _export(tmp_path, GPU)
+    before = launch_count()
+    _check_server(*_serve(tmp_path, "cuda:0", dtype=torch.bfloat16))
+    assert launch_count() > before
+    check_kernel_status(torch.device("cuda", 0))
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_gpu(tmp_path):
+    with pytest.raises(ValueError, match="head dimension of 128"):
+        PagedDecoder(_model(tmp_path / "a", {}, "cuda", torch.bfloat16))
+    with pytest.raises(ValueError, match="bfloat16 or float16"):
+        PagedDecoder(_model(tmp_path / "b", GPU, "cuda", torch.float32))
