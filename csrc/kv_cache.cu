@@ -113,8 +113,8 @@ constexpr int kHeads = 4;                    // key/value heads of a thread bloc
 // One block of 16 cached tokens (those of its tokens that are new) and up to four key/value heads with
 // their query heads.  Thread block b finds its tokens itself: sequence i has at most
 // new / 16 + 2 blocks, so the ones from cu[i] / 16 + 3 i on are its own, and a few stay empty.  After that
-// all loads are under way at once.  A team's items are dealt rows first: sixteen rows give every
-// team a row and all its heads, one row gives every team a head.
+// all loads are under way at once.  A team has one row: sixteen rows give it all heads of its row, one
+// row is shared by all teams, a head each.
 template <typename T>
 __global__ void __launch_bounds__(kAppendThreads, 3) cache_append_kernel(const AppendParams p) {
   __shared__ int at_row, at_pos, at_page, at_rows, at_written;  // first new row, its position, page, rows, rows written
@@ -186,39 +186,44 @@ __global__ void __launch_bounds__(kAppendThreads, 3) cache_append_kernel(const A
   const float* sin = p.sin + (int64_t)pos0 * kCacheDim + d;
   const int writes = page >= 0 ? written : 0;
 
-  // ---- keys and values: up to kHeads items a team, held until their scale is known
-  float4 klo[kHeads], khi[kHeads];
-  uint2 vr[kHeads][2];
+  // Team -> row r and the heads sub, sub + subs, ...: as many teams a row as a power of two allows.
+  const int shift = rows > 8 ? 4 : rows > 4 ? 3 : rows > 2 ? 2 : rows > 1 ? 1 : 0;
+  const int r = team & ((1 << shift) - 1), sub = team >> shift, subs = kTeams >> shift;
+  const bool writing = r < writes, reading = r < written;
+  const T* kr = k + r * p.k_tok;
+  const T* vr = v + r * p.v_tok;
+  const T* qr = q + r * p.q_tok;
+  // ---- keys and values, held as they are until their scale is known
+  uint2 kraw[kHeads][2], vraw[kHeads][2];
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    const int item = team + i * kTeams, r = item % rows, h = item / rows;
-    klo[i] = khi[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-    vr[i][0] = vr[i][1] = make_uint2(0, 0);
-    if (h < heads && r < writes) {
-      const T* ks = k + r * p.k_tok + h * p.k_head;
-      const T* vs = v + r * p.v_tok + h * p.v_head;
-      klo[i] = widen<T>(raw4(ks)), khi[i] = widen<T>(raw4(ks + 64));
-      vr[i][0] = raw4(vs), vr[i][1] = raw4(vs + 64);
+    const int h = sub + i * subs;
+    kraw[i][0] = kraw[i][1] = vraw[i][0] = vraw[i][1] = make_uint2(0, 0);
+    if (writing && h < heads) {
+      kraw[i][0] = raw4(kr + h * p.k_head), kraw[i][1] = raw4(kr + h * p.k_head + 64);
+      vraw[i][0] = raw4(vr + h * p.v_head), vraw[i][1] = raw4(vr + h * p.v_head + 64);
     }
+  }
+  float4 cl, ch, sl, sh;
+  cl = ch = sl = sh = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (reading) {
+    const float* c = cos + r * kCacheDim;
+    const float* s = sin + r * kCacheDim;
+    cl = *reinterpret_cast<const float4*>(c), ch = *reinterpret_cast<const float4*>(c + 64);
+    sl = *reinterpret_cast<const float4*>(s), sh = *reinterpret_cast<const float4*>(s + 64);
   }
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    const int item = team + i * kTeams, r = item % rows, h = item / rows;
-    if (i * kTeams >= rows * heads) break;  // the same for the whole block: the shuffles below are the warp's
-    const bool held = h < heads && r < writes;
-    if (held) {
-      const float* c = cos + r * kCacheDim;
-      const float* s = sin + r * kCacheDim;
-      rotate(klo[i], khi[i], *reinterpret_cast<const float4*>(c), *reinterpret_cast<const float4*>(c + 64),
-             *reinterpret_cast<const float4*>(s), *reinterpret_cast<const float4*>(s + 64));
-    }
+    const int h = sub + i * subs;
+    if (i * subs >= heads) break;  // the same for the whole block: the shuffles below are the warp's
+    const bool held = writing && h < heads;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      float4 lo = which ? widen<T>(vr[i][0]) : klo[i], hi = which ? widen<T>(vr[i][1]) : khi[i];
+      float4 lo = widen<T>(which ? vraw[i][0] : kraw[i][0]), hi = widen<T>(which ? vraw[i][1] : kraw[i][1]);
+      if (which == 0) rotate(lo, hi, cl, ch, sl, sh);
       bool bad = false;
       uint32_t top = take_finite(lo, bad);
       top = max(top, take_finite(hi, bad));
-      if (which == 0) klo[i] = lo, khi[i] = hi;
       if (bad && held) poisoned[h][which] = 1;
 #pragma unroll
       for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -226,21 +231,27 @@ __global__ void __launch_bounds__(kAppendThreads, 3) cache_append_kernel(const A
     }
   }
   // ---- queries, while the scales of the heads come together
-#pragma unroll 4
-  for (int item = team; item < rows * heads * group; item += kTeams) {
-    const int r = item % rows, h = item / rows;
-    float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
-    if (r < written) {
-      const T* src = q + r * p.q_tok + h * p.q_head;
-      const float* c = cos + r * kCacheDim;
-      const float* s = sin + r * kCacheDim;
-      lo = widen<T>(raw4(src)), hi = widen<T>(raw4(src + 64));
-      rotate(lo, hi, *reinterpret_cast<const float4*>(c), *reinterpret_cast<const float4*>(c + 64),
-             *reinterpret_cast<const float4*>(s), *reinterpret_cast<const float4*>(s + 64));
+  if (r < rows) {
+    T* dst = out + (int64_t)r * p.H * kCacheDim;
+    constexpr int kAhead = 4;
+    for (int base = sub; base < heads * group; base += kAhead * subs) {
+      uint2 w[kAhead][2];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int h = base + i * subs;
+        w[i][0] = w[i][1] = make_uint2(0, 0);
+        if (reading && h < heads * group) w[i][0] = raw4(qr + h * p.q_head), w[i][1] = raw4(qr + h * p.q_head + 64);
+      }
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) {
+        const int h = base + i * subs;
+        if (h >= heads * group) break;
+        float4 lo = widen<T>(w[i][0]), hi = widen<T>(w[i][1]);
+        rotate(lo, hi, cl, ch, sl, sh);
+        store4(dst + h * kCacheDim, lo);
+        store4(dst + h * kCacheDim + 64, hi);
+      }
     }
-    T* dst = out + ((int64_t)r * p.H + h) * kCacheDim;
-    store4(dst, lo);
-    store4(dst + 64, hi);
   }
   if (writes == 0) return;
   __syncthreads();
@@ -279,15 +290,17 @@ __global__ void __launch_bounds__(kAppendThreads, 3) cache_append_kernel(const A
   }
   __syncthreads();
   // ---- bytes
+  if (!writing) return;
 #pragma unroll
   for (int i = 0; i < kHeads; ++i) {
-    const int item = team + i * kTeams, r = item % rows, h = item / rows;
-    if (h >= heads || r >= writes) continue;
+    const int h = sub + i * subs;
+    if (h >= heads) break;
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      float4 lo = which ? widen<T>(vr[i][0]) : klo[i], hi = which ? widen<T>(vr[i][1]) : khi[i];
+      float4 lo = widen<T>(which ? vraw[i][0] : kraw[i][0]), hi = widen<T>(which ? vraw[i][1] : kraw[i][1]);
+      if (which == 0) rotate(lo, hi, cl, ch, sl, sh);
       bool bad;
-      if (which) take_finite(lo, bad), take_finite(hi, bad);
+      take_finite(lo, bad), take_finite(hi, bad);
       const float inv = two_to(-exponents[h][which]);  // -120 <= -e <= 32
       uint8_t* b = p.pages + (head_of(h, which) * p.page + in_page + r) * kCacheDim + d;
       *reinterpret_cast<uint32_t*>(b) = to_e4m3(times(lo, inv));

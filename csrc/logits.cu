@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(kThreads, 3) process_logits_kernel(const Logit
     prompt = p.prompt_lens != nullptr ? p.prompt_lens[row] : 0;
   }
   const float rep = p.repetition != nullptr ? p.repetition[row] : 1.f;
+  const float inv_rep = 1.f / rep;  // instead of a quotient a logit: one rounding more
   const float freq = p.frequency != nullptr ? p.frequency[row] : 0.f;
   const float pres = p.presence != nullptr ? p.presence[row] : 0.f;
   const bool counted = with_tokens || b1 > b0;
@@ -153,8 +154,8 @@ __global__ void __launch_bounds__(kThreads, 3) process_logits_kernel(const Logit
   }
   auto marked = [&](float v, uint32_t c) {
     const uint32_t made = c & kMadeMask;
-    if ((c & kSeen) || made) v = v > 0.f ? v / rep : v * rep;
-    if (made) v = v - freq * (float)made - pres;
+    if (c & (kSeen | kMadeMask)) v *= v > 0.f ? inv_rep : rep;
+    if (made) v -= fmaf(freq, (float)made, pres);
     if (c & kBiased) v += hit_values[c >> kHitShift & (kThreads - 1)];
     return v;
   };
