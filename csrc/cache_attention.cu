@@ -280,6 +280,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
     tma_prefetch_desc(&map);
     scan_base = 0;
   }
+  after_previous();
   // ---- the line of units
   for (int base = 0; base < p.n; base += kThreads) {
     const int i = base + (int)threadIdx.x;
@@ -682,8 +683,7 @@ cudaError_t launch(const CUtensorMap& map, const Params& p, int grid, cudaStream
     set[dev] = true;
   }
   grid = std::min(grid, Shape<kTiles>::kBlocksPerSm * 148);
-  cache_attention_kernel<T, kTiles><<<grid, kThreads, smem_bytes<kTiles>(), stream>>>(map, p);
-  return cudaGetLastError();
+  return launch_after_previous(cache_attention_kernel<T, kTiles>, grid, kThreads, smem_bytes<kTiles>(), stream, map, p);
 }
 
 }  // namespace

@@ -190,6 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int kvh = blockIdx.x % p.KV, group = p.group;
   const int tokens = kTile / group, per = 2 * tokens;  // tokens of a tile, and of this block
 
+  after_previous();
   // Sequence i has at most new / per + 1 blocks: those from cu[i] / per + 2 i on are its own, and some stay
   // empty.  The last blocks, which see most in a causal sequence, come first.
   const int last = gridDim.x / p.KV - 1, b = last - blockIdx.x / p.KV;
@@ -640,8 +641,7 @@ cudaError_t launch(const CUtensorMap& map_q, const CUtensorMap& map_pages, const
   const int per = 2 * (kTile / p.group);
   const int64_t grid = (int64_t)p.KV * (p.tokens / per + 2 * p.n + 1);
   if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-  cache_prompt_kernel<kBf16><<<(unsigned)grid, kThreads, kSmemBytes, stream>>>(map_q, map_pages, p);
-  return cudaGetLastError();
+  return launch_after_previous(cache_prompt_kernel<kBf16>, dim3((unsigned)grid), kThreads, kSmemBytes, stream, map_q, map_pages, p);
 }
 
 }  // namespace

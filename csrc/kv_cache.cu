@@ -108,19 +108,20 @@ __device__ __forceinline__ uint32_t take_finite(float4& v, bool& bad) {
 
 constexpr int kAppendThreads = 256;
 constexpr int kTeams = kAppendThreads / 16;  // a team of 16 lanes holds one row of a head
-constexpr int kHeads = 4;                    // key/value heads of a thread block
+constexpr int kHeads = 2;                    // key/value heads of a thread block
 
-// One block of 16 cached tokens (those of its tokens that are new) and up to four key/value heads with
+// One block of 16 cached tokens (those of its tokens that are new) and up to two key/value heads with
 // their query heads.  Thread block b finds its tokens itself: sequence i has at most
 // new / 16 + 2 blocks, so the ones from cu[i] / 16 + 3 i on are its own, and a few stay empty.  After that
 // all loads are under way at once.  A team has one row: sixteen rows give it all heads of its row, one
 // row is shared by all teams, a head each.
 template <typename T>
-__global__ void __launch_bounds__(kAppendThreads, 3) cache_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kAppendThreads, 4) cache_append_kernel(const AppendParams p) {
   __shared__ int at_row, at_pos, at_page, at_rows, at_written;  // first new row, its position, page, rows, rows written
   __shared__ uint32_t tops[kHeads][2];                          // largest magnitude, keys and values
   __shared__ int exponents[kHeads][2], poisoned[kHeads][2];
   const int lane = threadIdx.x & 31, team = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4;
+  after_previous();
   if (threadIdx.x < 32) {
     const int b = blockIdx.x;
     int lo = 0, size = p.n + 1;  // the last i with cu[i] / 16 + 3 i <= b, 32 candidates a step
@@ -312,8 +313,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) cache_append_kernel(const A
 template <typename T>
 cudaError_t launch_append(const AppendParams& p, cudaStream_t stream) {
   const dim3 grid(p.tokens / kCacheBlock + 3 * p.n + 1, (p.KV + kHeads - 1) / kHeads);
-  cache_append_kernel<T><<<grid, kAppendThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_after_previous(cache_append_kernel<T>, grid, kAppendThreads, 0, stream, p);
 }
 
 // ---------------------------------------------------------------------------------- pages
@@ -399,6 +399,7 @@ __global__ void __launch_bounds__(kBook) cache_reserve_kernel(int* table, int sl
   __shared__ int need[kMaxBatch];
   __shared__ int warp_sums[32];
   __shared__ int bad;
+  after_previous();
   if (threadIdx.x == 0) bad = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kBook) {
@@ -439,6 +440,7 @@ __global__ void __launch_bounds__(kBook) cache_reserve_kernel(int* table, int sl
 // Takes slot seqs[blockIdx.x]'s pages from it.
 __global__ void cache_free_kernel(int* table, int slots, int width, int* lens, int* refs, int npages, const int* seqs,
                                   int* status) {
+  after_previous();
   const int slot = seqs[blockIdx.x];
   if (slot < 0 || slot >= slots) {
     if (threadIdx.x == 0) report(status, kCacheBadSlot);
@@ -460,6 +462,7 @@ __global__ void __launch_bounds__(kBook) cache_fork_kernel(const Book b, const i
                                                            int* to, int* found, int* missing) {
   __shared__ int need[kMaxBatch];
   __shared__ int warp_sums[32];
+  after_previous();
   const int64_t entries = (int64_t)n * b.width;
   auto good = [&](int s, int d) { return s >= 0 && s < b.slots && d >= 0 && d < b.slots && s != d; };
   for (int64_t base = threadIdx.x; base < entries; base += 4 * kBook) {
@@ -547,6 +550,7 @@ __global__ void __launch_bounds__(kBook) cache_fork_kernel(const Book b, const i
 __global__ void __launch_bounds__(kBook) cache_plan_kernel(const int* refs, int npages, int* out_refs, int room, int* holes,
                                                            int* to, int* kept, int* missing) {
   __shared__ int warp_sums[32];
+  after_previous();
   int live = 0;
   for (int base = 0; base < npages; base += kBook * kPer) {
     int c = 0;
@@ -611,6 +615,7 @@ __device__ __forceinline__ bool copy_item(const CopyParams& p, int i, int& a, in
 
 // blockIdx.y: layer; blockIdx.x: a share of the list.
 __global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const CopyParams p) {
+  after_previous();
   if (p.missing != nullptr && *p.missing != 0) return;
   const int end = (int)(p.page_bytes / 16);
   for (int i = blockIdx.x; i < p.n; i += gridDim.x) {
@@ -655,34 +660,30 @@ cudaError_t launch_cache_append(const AppendParams& p, bool bf16, cudaStream_t s
 
 cudaError_t launch_cache_reserve(const Book& b, const int* seqs, const int* counts, int n, int* found, int* missing,
                                  cudaStream_t stream) {
-  cache_reserve_kernel<<<1, kBook, 0, stream>>>(b.table, b.slots, b.width, b.lens, b.refs, b.npages, seqs, counts, n, b.page,
-                                                found, missing);
-  return cudaGetLastError();
+  return launch_after_previous(cache_reserve_kernel, 1, kBook, 0, stream, b.table, b.slots, b.width, b.lens, b.refs, b.npages,
+                               seqs, counts, n, b.page, found, missing);
 }
 
 cudaError_t launch_cache_free(const Book& b, const int* seqs, int n, cudaStream_t stream) {
-  cache_free_kernel<<<n, 256, 0, stream>>>(b.table, b.slots, b.width, b.lens, b.refs, b.npages, seqs, b.status);
-  return cudaGetLastError();
+  return launch_after_previous(cache_free_kernel, n, 256, 0, stream, b.table, b.slots, b.width, b.lens, b.refs, b.npages, seqs,
+                               b.status);
 }
 
 cudaError_t launch_cache_fork(const Book& b, const int* src, const int* dst, int n, int* from, int* to, int* found,
                               int* missing, cudaStream_t stream) {
-  cache_fork_kernel<<<1, kBook, 0, stream>>>(b, src, dst, n, from, to, found, missing);
-  return cudaGetLastError();
+  return launch_after_previous(cache_fork_kernel, 1, kBook, 0, stream, b, src, dst, n, from, to, found, missing);
 }
 
 cudaError_t launch_cache_plan(const int* refs, int npages, int* out_refs, int room, int* holes, int* to, int* kept,
                               int* missing, cudaStream_t stream) {
-  cache_plan_kernel<<<1, kBook, 0, stream>>>(refs, npages, out_refs, room, holes, to, kept, missing);
-  return cudaGetLastError();
+  return launch_after_previous(cache_plan_kernel, 1, kBook, 0, stream, refs, npages, out_refs, room, holes, to, kept, missing);
 }
 
 cudaError_t launch_cache_copy(const CopyParams& p, cudaStream_t stream) {
   if (p.layers == 0 || (p.n == 0 && p.entries == 0)) return cudaSuccess;
   const int y = std::min(p.layers, 65535);
   const int x = std::min(std::max(p.n, 1), std::max(1, 148 * 8 / y));
-  cache_copy_kernel<<<dim3(x, y), kCopyThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_after_previous(cache_copy_kernel, dim3(x, y), kCopyThreads, 0, stream, p);
 }
 
 }  // namespace mimir

@@ -54,6 +54,7 @@ __global__ void __launch_bounds__(kThreads, 3) process_logits_kernel(const Logit
   const bool with_tokens = p.tokens != nullptr;
   const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld + v0;
   float* y = p.out + (int64_t)row * p.vocab + v0;
+  after_previous();
   Raw raw[kEach / 4];
   T single[kAligned ? 1 : kEach];
   if (kAligned) {
@@ -219,9 +220,8 @@ cudaError_t launch(const LogitsParams& p, cudaStream_t stream) {
   // Four logits at a time where every row starts on their boundary, and ends on one.
   const bool aligned = p.vocab % 4 == 0 && p.ld % 4 == 0 && reinterpret_cast<uintptr_t>(p.logits) % (4 * sizeof(T)) == 0 &&
                        reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
-  if (aligned) process_logits_kernel<T, true><<<grid, kThreads, 0, stream>>>(p);
-  else process_logits_kernel<T, false><<<grid, kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  return launch_after_previous(aligned ? process_logits_kernel<T, true> : process_logits_kernel<T, false>, grid, kThreads, 0,
+                               stream, p);
 }
 
 }  // namespace

@@ -7,6 +7,7 @@
 #include <algorithm>
 #include <map>
 #include <mutex>
+#include <tuple>
 
 #include "serving.h"
 #include "tma.cuh"
@@ -134,22 +135,36 @@ CUtensorMap queries_map(const at::Tensor& q, int64_t group) {
   return map;
 }
 
-// Counters that are zero before and after every call: kept per stream, whose calls follow one another;
-// a graph, which may run beside its stream, gets its own from its pool.
-int* arrival_counters(const at::Device& dev, cudaStream_t stream, at::Tensor& keep) {
+// Counters that are zero before and after every call, and room for partial sums.  Both are kept per stream, whose
+// calls follow one another.  A graph may run beside the stream that it was captured on: it has counters of
+// its own (per stream of the capture, cleared at its first call), and its partial sums come from its pool.
+struct AttentionParts {
+  float2 ml[kAttentionBlocks][2][kAttentionRows];
+  float sums[kAttentionBlocks][2][kAttentionRows][kCacheDim];
+};
+
+struct AttentionWork {
+  at::Tensor arrived, parts;
+};
+
+AttentionWork attention_work(const at::Device& dev, cudaStream_t stream) {
   cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-  C10_CUDA_CHECK(cudaStreamIsCapturing(stream, &capturing));
-  const auto options = at::TensorOptions().device(dev).dtype(at::kInt);
-  if (capturing != cudaStreamCaptureStatusNone) {
-    keep = at::zeros({kAttentionBlocks}, options);
-    return keep.data_ptr<int>();
-  }
+  unsigned long long capture = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream, &capturing, &capture));
+  if (capturing == cudaStreamCaptureStatusNone) capture = 0;  // captures count from one
+  const auto bytes = at::TensorOptions().device(dev).dtype(at::kByte);
   static std::mutex mutex;
-  static auto* kept = new std::map<std::pair<int, cudaStream_t>, at::Tensor>;  // never freed: it may outlive the context
+  // Never freed: the tensors may outlive the context, and nothing tells when a graph is gone (2 KB each).
+  static auto* kept = new std::map<std::tuple<int, cudaStream_t, unsigned long long>, AttentionWork>;
   std::lock_guard<std::mutex> lock(mutex);
-  at::Tensor& t = (*kept)[{dev.index(), stream}];
-  if (!t.defined()) t = at::zeros({kAttentionBlocks}, options);
-  return t.data_ptr<int>();
+  AttentionWork& work = (*kept)[{dev.index(), stream, capture}];
+  if (!work.arrived.defined()) {
+    work.arrived = at::empty({kAttentionBlocks * (int64_t)sizeof(int)}, bytes);
+    C10_CUDA_CHECK(cudaMemsetAsync(work.arrived.data_ptr(), 0, kAttentionBlocks * sizeof(int), stream));
+    if (capture == 0) work.parts = at::empty({(int64_t)sizeof(AttentionParts)}, bytes);
+  }
+  if (capture == 0) return work;
+  return {work.arrived, at::empty({(int64_t)sizeof(AttentionParts)}, bytes)};
 }
 
 const at::Tensor* given(const c10::optional<at::Tensor>& t) { return t.has_value() ? &*t : nullptr; }
@@ -375,8 +390,11 @@ at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at
     return out;
   }
   const CUtensorMap map = pages_map(pages, kAttentionKeys);
-  at::Tensor keep;
-  p.arrived = arrival_counters(dev, stream, keep);
+  const AttentionWork work = attention_work(dev, stream);
+  auto* parts = static_cast<AttentionParts*>(work.parts.data_ptr());
+  p.arrived = static_cast<int*>(work.arrived.data_ptr());
+  p.parts = &parts->sums[0][0][0][0];
+  p.part_ml = &parts->ml[0][0][0];
   const bool full = max_new < 1 || max_new * p.group > 8;
   for (int64_t base = 0; base < n; base += kAttentionSeqs) {
     p.n = (int)std::min<int64_t>(kAttentionSeqs, n - base);
@@ -388,9 +406,6 @@ at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at
     const int64_t segments = std::min<int64_t>(q.size(0), p.n) + q.size(0) * p.group / kAttentionRows + 1;
     const int64_t most = segments * KV * (((int64_t)p.width * p.page + kAttentionKeys - 1) / kAttentionKeys + 1 + kAttentionEnds);
     const int grid = (int)std::min<int64_t>(kAttentionBlocks, std::max<int64_t>(most, 1));
-    at::Tensor work = at::empty({grid * (int64_t)(2 * kAttentionRows * (kCacheDim + 2))}, q.options().dtype(at::kFloat));
-    p.parts = work.data_ptr<float>();
-    p.part_ml = reinterpret_cast<float2*>(p.parts + (int64_t)grid * 2 * kAttentionRows * kCacheDim);
     C10_CUDA_CHECK(launch_cache_attention(map, p, bf16, full, grid, stream));
   }
   return out;

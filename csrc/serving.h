@@ -31,6 +31,29 @@ enum CacheStatus : int {
   kCacheTimeout = 4,    // a wait inside a kernel ran out
 };
 
+// Launches on `stream` so that the kernel is set up while the one before it ends: 1.2 to 2.4 us less a call of
+// cache_attention.  The kernel calls after_previous() before it touches global memory: there it waits until
+// all that came before is done and visible.  (Letting the next kernel start earlier than at a kernel's end
+// cost the larger calls 1 us: its blocks wait where this one's could run.)
+template <typename... P, typename... A>
+inline cudaError_t launch_after_previous(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
+                                         const A&... args) {
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = grid;
+  config.blockDim = dim3(threads);
+  config.dynamicSmemBytes = smem;
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, P(args)...);
+}
+#ifdef __CUDACC__
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+#endif
+
 // ---------------------------------------------------------------- kv_cache.cu
 cudaError_t cache_status_address(void** word);  // of the current device
 
