@@ -43,7 +43,7 @@ struct Four<float> {
 };
 
 template <typename T, bool kAligned>
-__global__ void __launch_bounds__(kThreads, 3) process_logits_kernel(const LogitsParams p) {
+__global__ void __launch_bounds__(kThreads, 4) process_logits_kernel(const LogitsParams p) {
   __shared__ __align__(16) uint32_t counts[kSlice];
   __shared__ __align__(16) int hit_ids[kThreads + 4];
   __shared__ float hit_values[kThreads];

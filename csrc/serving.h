@@ -111,9 +111,9 @@ constexpr int kAttentionKeys = 64;         // keys of a unit
 constexpr int kAttentionRows = 16;         // query rows of a tile
 constexpr int kAttentionSeqs = 1024;       // sequences of one launch
 constexpr int kAttentionBlocks = 3 * 148;  // at most three blocks an SM
-// A segment's ends (queries in, results out) take as long as about three units of keys: its share of
+// A segment's ends (queries in, results out) take as long as some five units of keys: its share of
 // the line of work is that much longer, or blocks with many short segments would finish last.
-constexpr int kAttentionEnds = 3;
+constexpr int kAttentionEnds = 5;
 
 struct AttentionParams {
   const void* q;
