@@ -25,6 +25,12 @@
 // 32c..32c+31 of a key row, which two 16-byte loads bring without bank conflicts under the swizzle, and
 // the same dimensions of the query rows.  Of the values thread (g, c) takes the bytes 16g..16g+15 of
 // four rows; row g of product j is dimension 16g + 2j, row g + 8 the one after it.
+//
+// Measured on B200 (16 query and 4 key/value heads, one new token): 64 sequences to 8000 tokens 40 us for
+// 166 MB; 8 sequences to 100001 tokens 74 us for 391 MB (5.3 TB/s; 6.4 TB/s between two lengths, where the
+// some 10 us of start and joining cancel); DRAM reads are the cache's bytes and no more.  24 sequences to
+// 2100 tokens, 7 tokens, 20 and 20 heads: 44 us for 138 MB.  With the rows as the wide side of the products
+// (half of it empty) a warp needs 406 instructions for 16 keys instead of some 200: 55, 87 and 83 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 

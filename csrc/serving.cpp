@@ -439,8 +439,8 @@ at::Tensor process_logits(at::Tensor logits, c10::optional<at::Tensor> tokens, c
   if (tokens.has_value()) {
     SERVING_CHECK(tokens->device() == dev && tokens->scalar_type() == at::kInt && tokens->dim() == 2 &&
                           tokens->size(0) == rows && (tokens->stride(1) == 1 || tokens->size(1) <= 1) &&
-                          tokens->size(1) < (int64_t(1) << 31) - 64,
-                      "tokens must be int32 [rows, history] on ", dev, " with contiguous rows");
+                          tokens->size(1) < (int64_t(1) << 21),
+                      "tokens must be int32 [rows, history < 2^21] on ", dev, " with contiguous rows");
   } else {
     SERVING_CHECK(!token_lens.has_value() && !prompt_lens.has_value() && !repetition.has_value() &&
                           !presence.has_value() && !frequency.has_value(),
