@@ -15,7 +15,7 @@
 //
 // Pages.  One block keeps the books (sums over the batch, free pages lowest first by a scan of the counts), so
 // that results do not depend on scheduling; a second launch moves the bytes.  4 prompts forked to 32 slots over 24
-// layers: 17 us, of it some 5 for the books, for 50 MB written; 292 pages of 24 layers into another pool: 110 us
+// layers: 17 us, of it some 5 for the books, for 50 MB written; 195 pages of 24 layers into another pool: 110 us
 // (5.5 TB/s read and written).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

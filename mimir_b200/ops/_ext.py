@@ -15,7 +15,7 @@ _LOAD_ERROR: Exception | None = None
 
 # Kernel launches issued by one call of each binding (for launch accounting in benchmarks).
 _LAUNCHES_PER_CALL = {"fmha_status": 0, "fmha_plan": 1, "gemm_status": 0, "grouped_gemm_status": 0,
-                      "cache_status": 0, "cache_attention": 2, "cache_fork": 3, "cache_compact": 4}
+                      "cache_status": 0, "cache_fork": 2, "cache_compact": 2}
 
 
 class _CountingModule:

@@ -498,3 +498,33 @@ def test_logits_against_the_rules(rows, vocab, dtype):
         want = ops.process_logits(y, **kw)
         assert ops.process_logits(y, **kw, out=y) is not None
         torch.testing.assert_close(y, want, rtol=0, atol=0, equal_nan=True)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [1, 2, 5, 31, 8190, 8191, 8193, 16383])
+def test_logits_of_rows_that_start_anywhere(vocab, dtype):
+    gen = torch.Generator(DEV).manual_seed(vocab)
+    rows = 5
+    x = (3 * torch.randn(rows, vocab, generator=gen, device=DEV)).to(dtype)
+    tokens = torch.randint(-2, vocab + 3, (rows, 300), generator=gen, device=DEV).to(torch.int32)
+    ids = torch.randint(-2, vocab + 3, (rows * 600,), generator=gen, device=DEV).to(torch.int32)  # more than threads
+    kw = dict(tokens=tokens, token_lens=ints([300, 0, 7, 299, 1]).to(DEV), prompt_lens=ints([100, 0, 3, 299, 0]).to(DEV),
+              repetition=torch.rand(rows, generator=gen, device=DEV) + 0.5, presence=torch.rand(rows, generator=gen, device=DEV),
+              frequency=torch.rand(rows, generator=gen, device=DEV),
+              bias=(ints([0, 600, 1200, 1200, 2400, 3000]).to(DEV), ids, torch.randn(rows * 600, generator=gen, device=DEV)),
+              allowed=torch.randint(-2 ** 31, 2 ** 31, (rows, -(-vocab // 32)), generator=gen, device=DEV).to(torch.int32))
+    want = torch.full((rows, vocab), math.nan, device=DEV)
+    ref = process_logits_reference(x.double(), *(kw[k] for k in (
+        "tokens", "token_lens", "prompt_lens", "repetition", "presence", "frequency")), *kw["bias"], kw["allowed"])
+    ops.process_logits(x, **kw, out=want)
+    # a quotient, three sums and up to 1200 biases under 2^3, each rounded to 2^-24 of sizes under 2^13
+    torch.testing.assert_close(want, ref.float(), rtol=2.0 ** -21, atol=1204 * 2.0 ** -24 * 2.0 ** 13)
+    for stride, first, before in ((vocab, 1, 0), (vocab, 1, 1), (vocab + 1, 0, 0), (vocab + 2, 3, 2), (vocab + 3, 2, 3),
+                                  (vocab + 4, 0, 1)):
+        around = torch.full((stride * rows + first + 8,), math.nan, device=DEV, dtype=dtype)
+        view = around[first:first + stride * rows].view(rows, stride)[:, :vocab]
+        view.copy_(x)
+        out = torch.full((before + rows * vocab + 8,), 77.0, device=DEV)
+        got = ops.process_logits(view, **kw, out=out[before:before + rows * vocab].view(rows, vocab))
+        assert torch.equal(got, want), (stride, first, before)
+        assert (out[:before] == 77).all() and (out[before + rows * vocab:] == 77).all()
