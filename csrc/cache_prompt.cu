@@ -25,7 +25,8 @@
 // 128 keys a tile (the same columns), scores to P to products is a chain that leaves the tensor
 // cores idle for more than half of the time; with two of 64 the next scores are there when a softmax ends.
 // Measured on B200: five prompts to 4096 tokens (13703 in all), 16 and 4 heads, every token sees its whole
-// prompt: 416 us, 824 TFLOP/s of 1641; tensor pipe active 41 %.  (One S of 128 keys a tile: 489 us; one MMA
+// prompt: 392 us, 876 TFLOP/s of 1641; tensor pipe active 44 %.  Products alone, without the softmax's work, take
+// 350 us of it, the softmax beside half of the products 401 (before the order of blocks below: 416).  (One S of 128 keys a tile: 489 us; one MMA
 // warp for both tiles: 478 us, since issuing takes as long as the products; softmax rows on two warps: 473 us.)
 // O is rescaled only when a row's maximum grows by more than 2^8; only then is the last product
 // waited for.  Registers: 512 threads start with 128 each; the softmax groups take 184, the converters
@@ -194,21 +195,43 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int tokens = kTile / group, per = 2 * tokens;  // tokens of a tile, and of this block
 
   after_previous();
-  // Sequence i has at most new / per + 1 blocks: those from cu[i] / per + 2 i on are its own, and some stay
-  // empty.  The last blocks, which see most in a causal sequence, come first.
-  const int last = gridDim.x / p.KV - 1, b = last - blockIdx.x / p.KV;
-  int lo = 0, size = p.n + 1;
-  while (size > 1) {
-    const int step = (size + 31) / 32;
-    const int at = min(lo + lane * step, p.n);
-    const int c = __popc(__ballot_sync(0xffffffffu, lo + lane * step < lo + size && p.cu[at] / per + 2 * at <= b));
-    const int next = lo + max(c - 1, 0) * step;
-    size = min(step, lo + size - next);
-    lo = next;
+  const int last = gridDim.x / p.KV - 1;
+  int lo, tok0;  // this block's sequence (p.n: none) and first token in it
+  if (p.n <= 32) {
+    // Blocks of the longest sequences come first, within a sequence those of its last tokens, which see most where
+    // it is causal: the GPU's last blocks are then short ones (five prompts of 1343 to 4096 tokens: 416 -> 392 us).
+    // Lane i has sequence i.
+    const int at = min(lane, p.n), from = p.cu[at], slot = at < p.n ? p.seqs[at] : -1;
+    const int keys = slot >= 0 && slot < p.slots ? p.lens[slot] : 0;
+    const int news = at < p.n && from >= 0 ? max(min(p.cu[at + 1], p.tokens) - from, 0) : 0;
+    const int blocks = (news + per - 1) / per;
+    int before = 0;
+    for (int i = 0; i < p.n; ++i) {
+      const int keys_i = __shfl_sync(0xffffffffu, keys, i), blocks_i = __shfl_sync(0xffffffffu, blocks, i);
+      if (keys_i > keys || (keys_i == keys && i < lane)) before += blocks_i;
+    }
+    const int mine = before + blocks - 1 - (int)(blockIdx.x / p.KV);
+    const uint32_t owner = __ballot_sync(0xffffffffu, mine >= 0 && mine < blocks);
+    lo = owner != 0 ? __ffs(owner) - 1 : p.n;
+    tok0 = __shfl_sync(0xffffffffu, mine, lo & 31) * per;
+  } else {
+    // Sequence i has at most new / per + 1 blocks: those from cu[i] / per + 2 i on are its own, and some stay
+    // empty.  The last ones come first.
+    const int b = last - blockIdx.x / p.KV;
+    lo = 0;
+    for (int size = p.n + 1; size > 1;) {
+      const int step = (size + 31) / 32;
+      const int at = min(lo + lane * step, p.n);
+      const int c = __popc(__ballot_sync(0xffffffffu, lo + lane * step < lo + size && p.cu[at] / per + 2 * at <= b));
+      const int next = lo + max(c - 1, 0) * step;
+      size = min(step, lo + size - next);
+      lo = next;
+    }
+    tok0 = lo < p.n ? (b - (p.cu[lo] / per + 2 * lo)) * per : 0;
   }
   if (lo >= p.n) {
-    // rows that belong to no sequence: one block per head clears them
-    if (b == last && p.last_batch) {
+    // rows that belong to no sequence: one block per head, which has never any of its own, clears them
+    if (blockIdx.x / p.KV == (p.n <= 32 ? last : 0) && p.last_batch) {
       const int from = min(max(p.cu[p.n], 0), p.tokens);
       uint4* o = reinterpret_cast<uint4*>(p.out);
       constexpr int kWords = kCacheDim * 2 / 16;
@@ -220,7 +243,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     return;
   }
   const int first_row = p.cu[lo], count = first_row < 0 ? 0 : max(min(p.cu[lo + 1], p.tokens) - first_row, 0);
-  const int tok0 = (b - (first_row / per + 2 * lo)) * per;
   if (tok0 < 0 || tok0 >= count) return;  // block-uniform, before any allocation
   const int slot = p.seqs[lo], prefix = p.prefix != nullptr ? p.prefix[lo] : 0;
   int len = 0;

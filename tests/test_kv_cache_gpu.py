@@ -154,6 +154,16 @@ def test_many_short_prompts():
     check_attention(st, list(range(1100)), counts, 4, kernel=2)
 
 
+@pytest.mark.parametrize("many", [1, 31, 32, 33])
+def test_prompts_in_the_order_of_their_lengths(many):
+    """Up to 32 sequences the prompt kernel takes the longest first; equal and empty ones among them."""
+    counts = [(i * 37) % 150 for i in range(many - 1)] + [90]
+    lens = [c + (i * 53) % 90 // 30 * 30 for i, c in enumerate(counts)]
+    st = filled([max(n, 1) for n in lens], 3, 32)
+    for prefix in (None, lens):
+        check_attention(st, list(range(many))[::-1], counts[::-1], 12, prefix=prefix and prefix[::-1], extra_rows=5, kernel=2)
+
+
 def test_results_do_not_depend_on_the_run():
     st = filled([5000, 77, 20000], 4, 64)
     q, first = check_attention(st, [0, 1, 2], [1, 1, 1], 16, max_new=1)
