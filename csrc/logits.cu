@@ -10,8 +10,8 @@
 // their time, so a block asks for all that it can at once: its logits, the row's first 4096 tokens
 // before it knows how many count, the biases before it knows which are its own.  It counts the row's
 // tokens that fall into its slice in shared memory (whole numbers, so the order of the atomics does not
-// matter); the few biases of the slice lie in a list, equal ids summed in their order, and a token's
-// word says which of them is its own.  The history is read by every block of a row, from L2 after the
+// matter); a token's word also says which bias is its own, and where an id has several, a warp sums them
+// in their order.  The history is read by every block of a row, from L2 after the
 // first, so slices are large.
 //
 // Rows need not start on a boundary of four logits (an odd vocabulary, a view of padded logits): a slice
@@ -60,9 +60,9 @@ enum Rows { kRowsAligned, kRowsAlike, kRowsOther };
 template <typename T, Rows kRows>
 __global__ void __launch_bounds__(kThreads, kRows == kRowsAligned ? 4 : 3) process_logits_kernel(const LogitsParams p) {
   __shared__ __align__(16) uint32_t counts[kSlice];
-  __shared__ __align__(16) int hit_ids[kThreads + 4];
+  __shared__ int hit_ids[kThreads], again[kThreads];  // a thread's bias; ids that came again
   __shared__ float hit_values[kThreads];
-  __shared__ int warp_hits[kThreads / 32];
+  __shared__ int repeats;
   using Raw = typename Four<T>::Raw;
   const int row = blockIdx.y, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   // The slice: the row's logits v0 + i, lo <= i < here; where i is a multiple of four, they lie on the boundary.
@@ -122,28 +122,17 @@ __global__ void __launch_bounds__(kThreads, kRows == kRowsAligned ? 4 : 3) proce
   const float freq = p.frequency != nullptr ? p.frequency[row] : 0.f;
   const float pres = p.presence != nullptr ? p.presence[row] : 0.f;
   const bool counted = with_tokens || b1 > b0;
-  int hits = 0;
   if (counted) {
     const int bias_id = b0 + tid < b1 ? p.bias_ids[b0 + tid] - v0 : 0;
     const float bias = b0 + tid < b1 ? p.bias_values[b0 + tid] : 0.f;
     const bool hit = b0 + tid < b1 && inside(bias_id);
 #pragma unroll
     for (int i = 0; i < kEach / 4; ++i) reinterpret_cast<uint4*>(counts)[i * kThreads + tid] = make_uint4(0, 0, 0, 0);
-    const uint32_t mask = __ballot_sync(0xffffffffu, hit);
-    if (lane == 0) warp_hits[warp] = __popc(mask);
+    hit_ids[tid] = hit ? bias_id : -1;
+    hit_values[tid] = bias;
+    if (tid == 0) repeats = 0;
     __syncthreads();
-    int before = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      if (w < warp) before += warp_hits[w];
-      hits += warp_hits[w];
-    }
-    if (hit) {
-      const int k = before + __popc(mask & ((1u << lane) - 1));
-      hit_ids[k] = bias_id;
-      hit_values[k] = bias;
-    }
-    if (tid < 4) hit_ids[hits + tid] = -1;
+    if (hit && atomicOr(&counts[bias_id], kBiased | (uint32_t)tid << kHitShift) & kBiased) again[atomicAdd(&repeats, 1)] = bias_id;
     auto count = [&](int id, int i) {
       const int at = id - v0;
       if (i < n && inside(at)) {
@@ -155,31 +144,29 @@ __global__ void __launch_bounds__(kThreads, kRows == kRowsAligned ? 4 : 3) proce
     for (int u = 0; u < kAhead; ++u) count(held[u], u * kThreads + tid);
 #pragma unroll 4
     for (int i = kAhead * kThreads + tid; i < n; i += kThreads) count(ids[i], i);
-    if (hits > 0) {
-      __syncthreads();
-      if (tid < hits) {
-        const int id = hit_ids[tid];
-        int first = tid, others = 0;
-        for (int k = 0; k < hits; k += 4) {
-          const int4 h = *reinterpret_cast<const int4*>(hit_ids + k);
-          others += (h.x == id) + (h.y == id) + (h.z == id) + (h.w == id);
-          if (h.w == id) first = min(first, k + 3);
-          if (h.z == id) first = min(first, k + 2);
-          if (h.y == id) first = min(first, k + 1);
-          if (h.x == id) first = min(first, k);
+    __syncthreads();
+    // An id with several biases: a warp sums them in their order, and the first one's place holds the sum.
+    const int many = repeats;
+    for (int r = warp; r < many; r += kThreads / 32) {
+      const int id = again[r];
+      bool taken = false;
+      for (int k = lane; k < r; k += 32) taken |= again[k] == id;
+      if (__any_sync(0xffffffffu, taken)) continue;
+      int first = -1;
+      float sum = 0.f;
+      for (int base = 0; base < kThreads; base += 32)
+        for (uint32_t m = __ballot_sync(0xffffffffu, hit_ids[base + lane] == id); m; m &= m - 1) {
+          const int k = base + __ffs(m) - 1;
+          if (first < 0) first = k;
+          sum += hit_values[k];
         }
-        if (first == tid) {
-          atomicOr(&counts[id], kBiased | (uint32_t)tid << kHitShift);
-          if (others > 1) {
-            float sum = 0.f;
-            for (int k = tid; k < hits; ++k)
-              if (hit_ids[k] == id) sum += hit_values[k];
-            hit_values[tid] = sum;  // no other thread sums this id
-          }
-        }
+      __syncwarp();
+      if (lane == 0) {
+        counts[id] = (counts[id] & (kSeen | kMadeMask)) | kBiased | (uint32_t)first << kHitShift;
+        hit_values[first] = sum;
       }
     }
-    __syncthreads();
+    if (many > 0) __syncthreads();
   }
   auto marked = [&](float v, uint32_t c) {
     const uint32_t made = c & kMadeMask;
