@@ -18,10 +18,10 @@
 // starts at the boundary before, and its first and last four may be partly another row's, which are
 // neither read nor written.
 //
-// Measured on B200: 128 rows of 65536 bf16 logits, up to 4000 tokens, 300 biases and a mask each: 18.6 us
-// for 53 MB (2.9 TB/s, issue slots 76 % full; without tokens, biases and mask 12 us); fp32 25 us; 65535
-// logits 23 us (28 with four blocks an SM, whose 32 registers such rows' edges spill; one logit at a time
-// 39); 65535 of rows of 65536 25 us; one row 5 us, of which its start is most.
+// Measured on B200: 128 rows of 65536 bf16 logits, up to 4000 tokens, 300 biases and a mask each: 16.5 us
+// for 53 MB (3.2 TB/s; without tokens, biases and mask 11 us); fp32 21 us; 65535 logits 20 us (one logit at
+// a time 39); 65535 of rows of 65536 22 us; one row 5 us, of which its start is most.  Halves or doubles of
+// slice and block take 23 and 20 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -55,10 +55,12 @@ struct Four<float> {
 
 // How rows lie: on boundaries of four logits, in and out; as far from one in as out, so that four results are one
 // store; or in some other way: results go through shared memory and are stored one by one, a warp's together.
+// (fp32 rows of the last two kinds: three blocks an SM, since at four 32 registers spill: 22 us instead of 23.)
 enum Rows { kRowsAligned, kRowsAlike, kRowsOther };
 
 template <typename T, Rows kRows>
-__global__ void __launch_bounds__(kThreads, kRows == kRowsAligned ? 4 : 3) process_logits_kernel(const LogitsParams p) {
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && kRows != kRowsAligned ? 3 : 4)
+    process_logits_kernel(const LogitsParams p) {
   __shared__ __align__(16) uint32_t counts[kSlice];
   __shared__ int hit_ids[kThreads], again[kThreads];  // a thread's bias; ids that came again
   __shared__ float hit_values[kThreads];
