@@ -25,9 +25,10 @@
 // 128 keys a tile (the same columns), scores to P to products is a chain that leaves the tensor
 // cores idle for more than half of the time; with two of 64 the next scores are there when a softmax ends.
 // Measured on B200: five prompts to 4096 tokens (13703 in all), 16 and 4 heads, every token sees its whole
-// prompt: 392 us, 876 TFLOP/s of 1641; tensor pipe active 39 % under the profiler (430 us there).  Products alone, without the softmax's work, take
-// 350 us of it, the softmax beside half of the products 401 (before the order of blocks below: 416).  (One S of 128 keys a tile: 489 us; one MMA
-// warp for both tiles: 478 us, since issuing takes as long as the products; softmax rows on two warps: 473 us.)
+// prompt: 392 us, 876 TFLOP/s of 1641; tensor pipe active 39 % under the profiler (430 us there).  What
+// bounds it: the products with next to nothing between them take 350 us, the softmax with half of the
+// products 401 (both before the order of blocks below, 416).  One S of 128 keys a tile: 489 us; one MMA warp
+// for both tiles: 478 us, since issuing takes as long as the products; a row's softmax on two warps: 473 us.
 // O is rescaled only when a row's maximum grows by more than 2^8; only then is the last product
 // waited for.  Registers: 512 threads start with 128 each; the softmax groups take 184, the converters
 // keep 88 and the producer and MMA group 56 (the sum is the same).

@@ -465,8 +465,12 @@ at::Tensor process_logits(at::Tensor logits, c10::optional<at::Tensor> tokens, c
     SERVING_CHECK(out->device() == dev && out->scalar_type() == at::kFloat && out->is_contiguous() &&
                           out->sizes() == logits.sizes(),
                       "out must be contiguous float32 of the logits' shape on ", dev);
-    SERVING_CHECK(out->data_ptr() != logits.data_ptr() || (type == at::kFloat && logits.is_contiguous()),
-                      "out may be the logits only where they are contiguous float32");
+    const char* a = static_cast<const char*>(logits.data_ptr());
+    const char* b = static_cast<const char*>(out->data_ptr());
+    const bool apart = rows == 0 || vocab == 0 || b + out->nbytes() <= a ||
+                       a + ((rows - 1) * logits.stride(0) + vocab) * logits.element_size() <= b;
+    SERVING_CHECK(apart || (a == b && type == at::kFloat && logits.is_contiguous()),
+                      "out may be the logits only where they are contiguous float32, and else shares no memory with them");
     y = *out;
   } else {
     y = at::empty({rows, vocab}, logits.options().dtype(at::kFloat));

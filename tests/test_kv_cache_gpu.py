@@ -538,3 +538,13 @@ def test_logits_of_rows_that_start_anywhere(vocab, dtype):
         got = ops.process_logits(view, **kw, out=out[before:before + rows * vocab].view(rows, vocab))
         assert torch.equal(got, want), (stride, first, before)
         assert (out[:before] == 77).all() and (out[before + rows * vocab:] == 77).all()
+
+
+def test_logits_out_that_overlaps_is_refused():
+    memory = torch.zeros(64, device=DEV)
+    x = memory[:40].view(2, 20)
+    with pytest.raises(ValueError, match="shares no memory"):
+        ops.process_logits(x, out=memory[4:44].view(2, 20))
+    with pytest.raises(ValueError, match="shares no memory"):
+        ops.process_logits(memory.view(torch.bfloat16)[:40].view(2, 20), out=memory[:40].view(2, 20))
+    ops.process_logits(x[:, :10], out=memory[40:60].view(2, 10))
