@@ -253,6 +253,8 @@ __device__ void join_parts(const Params& p, const Segment& sg, const Seq& s, int
   }
 }
 
+constexpr int kFewBlocks = 96;  // one sequence of 1000 keys: 84 blocks 10.5 us, 37 blocks 11.7
+
 template <typename T, int kTiles>
 __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -317,7 +319,12 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
     for (int64_t k = from * per + blockIdx.x * (int64_t)kThreads + threadIdx.x; k < p.tokens * per; k += (int64_t)gridDim.x * kThreads)
       o[k] = make_uint4(0, 0, 0, 0);
   }
-  const int64_t blocks = min((int64_t)gridDim.x, total);
+  // A unit takes about four times as long as joining a part does, and the last block of a segment joins all of its
+  // parts: few long segments are shared by fewer blocks, so that units / blocks + parts / 4 is least, but by
+  // kFewBlocks where there are units for them.  One sequence, 4 key/value heads, in us, with all blocks and so:
+  // 6128 keys 20.4, 12.9; 24000 keys 25.3, 21.1; three of 6128 keys 21.9, 19.6.
+  const int64_t best = max((int64_t)sqrtf((float)total * p.join_cost), (int64_t)kFewBlocks);
+  const int64_t blocks = min(min((int64_t)gridDim.x, total), best);
   if (blockIdx.x >= blocks) return;
   auto share = [&](int64_t b) {
     return total < (1 << 22) ? (int64_t)((uint32_t)(total * b) / (uint32_t)blocks) : total * b / blocks;

@@ -401,6 +401,7 @@ at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at
     p.seqs = seqs.data_ptr<int>() + base;
     p.cu = cu_new.data_ptr<int>() + base;
     p.prefix = prefix_lens.has_value() ? prefix_lens->data_ptr<int>() + base : nullptr;
+    p.join_cost = 4.f * (float)row_tiles * (float)p.n / (float)n;
     p.last_batch = base + p.n == n;
     // no more blocks than units: at most this many
     const int64_t segments = std::min<int64_t>(q.size(0), p.n) + q.size(0) * p.group / kAttentionRows + 1;

@@ -126,6 +126,7 @@ struct AttentionParams {
   int* arrived;         // per block: parts of the segment that it begins, zero between calls
   float* parts;         // [blocks][2][rows of a tile][128]
   float2* part_ml;      // [blocks][2][rows of a tile]: maximum and sum
+  float join_cost;      // four times the segments that the sequences have, about
   int last_batch;       // the call's last launch: rows that belong to no sequence become zeros
   int* status;
 };
