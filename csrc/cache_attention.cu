@@ -321,10 +321,14 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
   }
   // A unit takes about four times as long as joining a part does, and the last block of a segment joins all of its
   // parts: few long segments are shared by fewer blocks, so that units / blocks + parts / 4 is least, but by
-  // kFewBlocks where there are units for them.  One sequence, 4 key/value heads, in us, with all blocks and so:
-  // 6128 keys 20.4, 12.9; 24000 keys 25.3, 21.1; three of 6128 keys 21.9, 19.6.
+  // kFewBlocks where there are units for them, and with whole units a block.  One sequence, 4 key/value heads, in
+  // us, with all blocks and so: 6128 keys 20.4, 13.1; 24000 keys 25.3, 20.4; three of 6128 keys 21.9, 20.1.
   const int64_t best = max((int64_t)sqrtf((float)total * p.join_cost), (int64_t)kFewBlocks);
-  const int64_t blocks = min(min((int64_t)gridDim.x, total), best);
+  int64_t blocks = min((int64_t)gridDim.x, total);
+  if (best < blocks) {  // total < blocks^2 / 4 then
+    const uint32_t each = (uint32_t)total / (uint32_t)best;
+    blocks = min(blocks, (int64_t)(((uint32_t)total + each - 1) / each));
+  }
   if (blockIdx.x >= blocks) return;
   auto share = [&](int64_t b) {
     return total < (1 << 22) ? (int64_t)((uint32_t)(total * b) / (uint32_t)blocks) : total * b / blocks;
