@@ -46,7 +46,7 @@ namespace {
 constexpr int kKeys = kAttentionKeys;          // keys of a unit
 constexpr int kWarps = 4;                      // consumers
 constexpr int kThreads = (kWarps + 1) * 32;
-constexpr int kRows = kAttentionRows;          // rows of a tile
+constexpr int kRows = kAttentionRows;          // rows of a full tile
 constexpr uint32_t kHalfStage = kKeys * kCacheDim;
 constexpr uint32_t kStageBytes = 2 * kHalfStage;
 constexpr int kOutLd = 132;                    // floats of a row in the join buffer
@@ -58,8 +58,9 @@ constexpr int kEnds = kAttentionEnds;
 
 using Params = AttentionParams;
 
-// kTiles: products' widths of 8 that hold the tile's rows.  Eight rows leave registers and shared
-// memory for three blocks an SM, sixteen for two.
+// kTiles: products' widths of 8 that make a row tile.  Eight rows leave registers and shared memory for three
+// blocks an SM, sixteen for two.  Either takes any number of rows a sequence: what the host believes of it
+// decides only which is faster.
 template <int kTiles>
 struct Shape {
   static constexpr int kRowsHeld = 8 * kTiles;
@@ -171,14 +172,17 @@ __device__ Seq load_seq(const Params& p, int i) {
   return s;
 }
 __device__ __forceinline__ int seq_tiles(const Seq& s) { return max((s.len + kKeys - 1) / kKeys, 1); }
+template <int kMine>  // rows of a tile
 __device__ __forceinline__ int seq_row_tiles(const Params& p, const Seq& s) {
-  return (s.count * p.group + kRows - 1) / kRows;
+  return (s.count * p.group + kMine - 1) / kMine;
 }
+template <int kMine>
 __device__ __forceinline__ int64_t seq_units(const Params& p, const Seq& s) {
-  return (int64_t)p.KV * seq_row_tiles(p, s) * (seq_tiles(s) + kEnds);
+  return (int64_t)p.KV * seq_row_tiles<kMine>(p, s) * (seq_tiles(s) + kEnds);
 }
 
 // A block's share of the line, one segment at a time.
+template <int kMine>
 struct Walk {
   const Params& p;
   const Seq* window;   // sequences from `from` on: what a block's share meets, as a rule
@@ -189,11 +193,11 @@ struct Walk {
   __device__ bool next(Segment& g) {
     while (u < end) {
       int64_t units;
-      while (base + (units = seq_units(p, s)) <= u) {
+      while (base + (units = seq_units<kMine>(p, s)) <= u) {
         base += units;
         s = seq(++i);
       }
-      const int rts = seq_row_tiles(p, s);
+      const int rts = seq_row_tiles<kMine>(p, s);
       g.i = i;
       g.tiles = seq_tiles(s);
       const int length = g.tiles + kEnds;
@@ -222,7 +226,7 @@ struct Walk {
 };
 
 // Joins the parts of a segment, blocks b0 .. b1: a warp a row, a lane four columns.
-template <typename T>
+template <typename T, int kMine>
 __device__ void join_parts(const Params& p, const Segment& sg, const Seq& s, int rows, int b0, int b1, int warp, int lane) {
   auto part_of = [&](int b) { return (int64_t)b * 2 + (b == b0 ? 1 : 0); };
   for (int r = warp; r < rows; r += kWarps) {
@@ -247,7 +251,7 @@ __device__ void join_parts(const Params& p, const Segment& sg, const Seq& s, int
     }
     sum = warp_sum(sum);
     const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-    const int row = sg.rt * kRows + r;
+    const int row = sg.rt * kMine + r;
     T* dst = reinterpret_cast<T*>(p.out) + ((int64_t)(s.row + row / p.group) * p.H + sg.h * p.group + row % p.group) * kCacheDim;
     reinterpret_cast<uint2*>(dst)[lane] = make_uint2(Pair<T>::put(o.x * inv, o.y * inv), Pair<T>::put(o.z * inv, o.w * inv));
   }
@@ -259,7 +263,7 @@ template <typename T, int kTiles>
 __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr int kMine = Shape<kTiles>::kRowsHeld;  // rows of a tile that can hold queries
+  constexpr int kMine = Shape<kTiles>::kRowsHeld;  // rows of a tile
   constexpr int kStages = Shape<kTiles>::kStages;
   float* joined = reinterpret_cast<float*>(smem + kStages * kStageBytes);        // [kWarps][kMine][kOutLd]
   float* stats = joined + kWarps * kMine * kOutLd;                               // [kWarps][kMine][4]: m, M, l
@@ -292,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
   // ---- the line of units
   for (int base = 0; base < p.n; base += kThreads) {
     const int i = base + (int)threadIdx.x;
-    const int64_t units = i < p.n ? seq_units(p, load_seq(p, i)) : 0;
+    const int64_t units = i < p.n ? seq_units<kMine>(p, load_seq(p, i)) : 0;
     int64_t v = units;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -333,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
   auto share = [&](int64_t b) {
     return total < (1 << 22) ? (int64_t)((uint32_t)(total * b) / (uint32_t)blocks) : total * b / blocks;
   };
-  Walk walk{p, window, 0, 0, 0, share(blockIdx.x), share(blockIdx.x + 1), Seq{}};
+  Walk<kMine> walk{p, window, 0, 0, 0, share(blockIdx.x), share(blockIdx.x + 1), Seq{}};
   {
     int lo = 0, hi = p.n - 1;  // the last sequence with first <= u (empty ones have no units)
     while (lo < hi) {
@@ -351,7 +355,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
 
   // The tiles that a row tile needs: keys up to the largest limit of its rows.
   auto tiles_needed = [&](const Seq& s, int rt) {
-    return (row_limit(s, min((rt * kRows + kRows - 1) / p.group, s.count - 1)) + kKeys - 1) / kKeys;
+    return (row_limit(s, min((rt * kMine + kMine - 1) / p.group, s.count - 1)) + kKeys - 1) / kKeys;
   };
   Segment sg;
 
@@ -364,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
       // query rows of the tile, 16 bytes a lane, zeros beyond the last
       if (turn >= 2 && !warp_wait(&bar->q_empty[turn & 1], ((turn >> 1) - 1) & 1, p.status, kCacheTimeout)) break;
       for (int x = lane; x < kMine * 16; x += 32) {
-        const int r = sg.rt * kRows + (x >> 4), tok = r / p.group;
+        const int r = sg.rt * kMine + (x >> 4), tok = r / p.group;
         const bool held = tok < s.count;
         const T* src = reinterpret_cast<const T*>(p.q);
         if (held) src += (int64_t)(s.row + tok) * p.q_tok + (sg.h * p.group + r % p.group) * p.q_head + (x & 15) * 8;
@@ -435,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
     if (ok) ok = warp_wait(&bar->q_full[turn & 1], (turn >> 1) & 1, p.status, kCacheTimeout);
     const Seq s = walk.s;
     const int t1 = min(cur.t1, tiles_needed(s, cur.rt));
-    const int rows = min(s.count * p.group - cur.rt * kRows, kRows);
+    const int rows = min(s.count * p.group - cur.rt * kMine, kMine);
     // Rows 8n + g, dimensions 32c .. 32c + 31, as the products' second operand; and of rows
     // 8n + 2c and 8n + 2c + 1, whose scores this thread gets, the factor and the limit.
     uint32_t qb[kTiles][8][2];
@@ -469,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         qs[n][y] = __shfl_sync(0xffffffffu, back, (2 * c + y) * 4);
-        const int tok = (cur.rt * kRows + 8 * n + 2 * c + y) / p.group;
+        const int tok = (cur.rt * kMine + 8 * n + 2 * c + y) / p.group;
         lim[n][y] = 0;
         if (tok < s.count) {
           lim[n][y] = row_limit(s, tok);
@@ -636,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
         }
       if (cur.t0 == 0 && cur.t1 == cur.tiles) {
         const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-        const int row = cur.rt * kRows + r;
+        const int row = cur.rt * kMine + r;
         uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) +
                                               ((int64_t)(s.row + row / p.group) * p.H + cur.h * p.group + row % p.group) * kCacheDim + d0);
 #pragma unroll
@@ -675,8 +679,8 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
     if (!(has_split >> x & 1) || last_of[x] < 0) continue;
     __threadfence();
     const Seq s = walk.seq(split[x].i);
-    const int rows = min(s.count * p.group - split[x].rt * kRows, kRows);
-    join_parts<T>(p, split[x], s, rows, last_of[x], block_of(split[x].first_tile + split[x].tiles - 1), warp, lane);
+    const int rows = min(s.count * p.group - split[x].rt * kMine, kMine);
+    join_parts<T, kMine>(p, split[x], s, rows, last_of[x], block_of(split[x].first_tile + split[x].tiles - 1), warp, lane);
   }
 }
 

@@ -395,16 +395,19 @@ at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at
   p.arrived = static_cast<int*>(work.arrived.data_ptr());
   p.parts = &parts->sums[0][0][0][0];
   p.part_ml = &parts->ml[0][0][0];
+  // Tiles of 8 rows are faster where they hold a sequence's rows, and right where they do not.
   const bool full = max_new < 1 || max_new * p.group > 8;
+  const int64_t tile = full ? kAttentionRows : 8;
+  const int64_t tiles = KV * std::max<int64_t>(n, (q.size(0) * p.group + tile - 1) / tile);
   for (int64_t base = 0; base < n; base += kAttentionSeqs) {
     p.n = (int)std::min<int64_t>(kAttentionSeqs, n - base);
     p.seqs = seqs.data_ptr<int>() + base;
     p.cu = cu_new.data_ptr<int>() + base;
     p.prefix = prefix_lens.has_value() ? prefix_lens->data_ptr<int>() + base : nullptr;
-    p.join_cost = 4.f * (float)row_tiles * (float)p.n / (float)n;
+    p.join_cost = 4.f * (float)tiles * (float)p.n / (float)n;
     p.last_batch = base + p.n == n;
     // no more blocks than units: at most this many
-    const int64_t segments = std::min<int64_t>(q.size(0), p.n) + q.size(0) * p.group / kAttentionRows + 1;
+    const int64_t segments = std::min<int64_t>(q.size(0), p.n) + q.size(0) * p.group / tile + 1;
     const int64_t most = segments * KV * (((int64_t)p.width * p.page + kAttentionKeys - 1) / kAttentionKeys + 1 + kAttentionEnds);
     const int grid = (int)std::min<int64_t>(kAttentionBlocks, std::max<int64_t>(most, 1));
     C10_CUDA_CHECK(launch_cache_attention(map, p, bf16, full, grid, stream));

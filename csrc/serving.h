@@ -108,7 +108,7 @@ cudaError_t launch_cache_copy(const CopyParams& p, cudaStream_t stream);
 
 // ---------------------------------------------------------------- cache_attention.cu
 constexpr int kAttentionKeys = 64;         // keys of a unit
-constexpr int kAttentionRows = 16;         // query rows of a tile
+constexpr int kAttentionRows = 16;         // query rows of a tile, at most (the kernel for few rows has 8)
 constexpr int kAttentionSeqs = 1024;       // sequences of one launch
 constexpr int kAttentionBlocks = 3 * 148;  // at most three blocks an SM
 // A segment's ends (queries in, results out) take as long as some five units of keys: its share of

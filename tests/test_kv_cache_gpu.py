@@ -548,3 +548,19 @@ def test_logits_out_that_overlaps_is_refused():
     with pytest.raises(ValueError, match="shares no memory"):
         ops.process_logits(memory.view(torch.bfloat16)[:40].view(2, 20), out=memory[:40].view(2, 20))
     ops.process_logits(x[:, :10], out=memory[40:60].view(2, 10))
+
+
+def stale(shape, dtype):
+    """Leaves a freed block of NaN of this size behind: what a kernel does not write shows."""
+    torch.full(shape, math.nan, dtype=dtype, device=DEV)
+
+
+@pytest.mark.parametrize("heads,kv", [(8, 2), (3, 1), (20, 20), (24, 2)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_hint_below_the_real_number_of_new_tokens(heads, kv, dtype):
+    """``max_new`` chooses a kernel and changes no result, whatever it says."""
+    counts, lens = [3, 1, 9, 40, 0, 2], [300, 1, 9, 5000, 7, 129]
+    st = filled(lens, kv, 32, seed=heads)
+    for hint in (1, 2, 9):
+        stale((sum(counts), heads, DIM), dtype)
+        check_attention(st, list(range(6)), counts, heads, dtype, max_new=hint, kernel=1)
