@@ -316,13 +316,14 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
   __syncthreads();
   const int64_t total = first[p.n];
   // rows that belong to no sequence
-  if (p.last_batch) {
-    const int from = p.n > 0 ? min(max(p.cu[p.n], 0), p.tokens) : 0;
+  auto clear_rows = [&](int64_t from, int64_t to) {
     uint4* o = reinterpret_cast<uint4*>(p.out);
     const int64_t per = (int64_t)p.H * kCacheDim * sizeof(T) / 16;
-    for (int64_t k = from * per + blockIdx.x * (int64_t)kThreads + threadIdx.x; k < p.tokens * per; k += (int64_t)gridDim.x * kThreads)
+    for (int64_t k = from * per + blockIdx.x * (int64_t)kThreads + threadIdx.x; k < to * per; k += (int64_t)gridDim.x * kThreads)
       o[k] = make_uint4(0, 0, 0, 0);
-  }
+  };
+  if (p.first_batch) clear_rows(0, min(p.cu[0], p.tokens));
+  if (p.last_batch) clear_rows(min(max(p.cu[p.n], 0), p.tokens), p.tokens);
   // A unit takes about four times as long as joining a part does, and the last block of a segment joins all of its
   // parts: few long segments are shared by fewer blocks, so that units / blocks + parts / 4 is least, but by
   // kFewBlocks where there are units for them, and with whole units a block.  One sequence, 4 key/value heads, in

@@ -232,14 +232,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   if (lo >= p.n) {
     // rows that belong to no sequence: one block per head, which has never any of its own, clears them
-    if (blockIdx.x / p.KV == (p.n <= 32 ? last : 0) && p.last_batch) {
-      const int from = min(max(p.cu[p.n], 0), p.tokens);
-      uint4* o = reinterpret_cast<uint4*>(p.out);
-      constexpr int kWords = kCacheDim * 2 / 16;
-      for (int64_t x = threadIdx.x; x < (int64_t)(p.tokens - from) * group * kWords; x += kThreads) {
-        const int64_t row = x / kWords;
-        o[((from + row / group) * p.H + kvh * group + row % group) * kWords + x % kWords] = make_uint4(0, 0, 0, 0);
-      }
+    if (blockIdx.x / p.KV == (p.n <= 32 ? last : 0)) {
+      auto clear_rows = [&](int from, int to) {
+        uint4* o = reinterpret_cast<uint4*>(p.out);
+        constexpr int kWords = kCacheDim * 2 / 16;
+        for (int64_t x = threadIdx.x; x < (int64_t)(to - from) * group * kWords; x += kThreads) {
+          const int64_t row = x / kWords;
+          o[((from + row / group) * p.H + kvh * group + row % group) * kWords + x % kWords] = make_uint4(0, 0, 0, 0);
+        }
+      };
+      if (p.first_batch) clear_rows(0, min(max(p.cu[0], 0), p.tokens));
+      if (p.last_batch) clear_rows(min(max(p.cu[p.n], 0), p.tokens), p.tokens);
     }
     return;
   }

@@ -176,12 +176,13 @@ __global__ void __launch_bounds__(kAppendThreads, 4) cache_append_kernel(const A
     (&tops[0][0])[threadIdx.x - 32] = 0;
     (&poisoned[0][0])[threadIdx.x - 32] = 0;
   }
-  if (blockIdx.x == gridDim.x - 1) {  // rows that belong to no sequence
-    const int from = p.n > 0 ? min(max(p.cu[p.n], 0), p.tokens) : 0;
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) {  // rows that belong to no sequence
     uint4* o = reinterpret_cast<uint4*>(p.q_out);
     const int64_t per = (int64_t)p.H * kCacheDim / 8;
-    if (blockIdx.y == 0)
-      for (int64_t x = from * per + threadIdx.x; x < p.tokens * per; x += kAppendThreads) o[x] = make_uint4(0, 0, 0, 0);
+    const int64_t before = (p.n > 0 ? min(p.cu[0], p.tokens) : 0) * per;
+    const int64_t from = (p.n > 0 ? min(max(p.cu[p.n], 0), p.tokens) : 0) * per;
+    for (int64_t x = threadIdx.x; x < before; x += kAppendThreads) o[x] = make_uint4(0, 0, 0, 0);
+    for (int64_t x = from + threadIdx.x; x < p.tokens * per; x += kAppendThreads) o[x] = make_uint4(0, 0, 0, 0);
   }
   __syncthreads();
   const int rows = at_rows, written = at_written, pos0 = at_pos, page = at_page;

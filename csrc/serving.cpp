@@ -384,6 +384,7 @@ at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at
       p.seqs = seqs.data_ptr<int>() + base;
       p.cu = cu_new.data_ptr<int>() + base;
       p.prefix = prefix_lens.has_value() ? prefix_lens->data_ptr<int>() + base : nullptr;
+      p.first_batch = base == 0;
       p.last_batch = base + p.n == n;
       C10_CUDA_CHECK(launch_cache_prompt(map_q, map_pages, p, bf16, stream));
     }
@@ -405,6 +406,7 @@ at::Tensor cache_attention(at::Tensor q, at::Tensor pages, at::Tensor scales, at
     p.cu = cu_new.data_ptr<int>() + base;
     p.prefix = prefix_lens.has_value() ? prefix_lens->data_ptr<int>() + base : nullptr;
     p.join_cost = 4.f * (float)tiles * (float)p.n / (float)n;
+    p.first_batch = base == 0;
     p.last_batch = base + p.n == n;
     // no more blocks than units: at most this many
     const int64_t segments = std::min<int64_t>(q.size(0), p.n) + q.size(0) * p.group / tile + 1;

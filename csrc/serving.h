@@ -127,7 +127,8 @@ struct AttentionParams {
   float* parts;         // [blocks][2][rows of a tile][128]
   float2* part_ml;      // [blocks][2][rows of a tile]: maximum and sum
   float join_cost;      // four times the segments that the sequences have, about
-  int last_batch;       // the call's last launch: rows that belong to no sequence become zeros
+  int first_batch;      // the call's first launch: rows before all sequences become zeros
+  int last_batch;       // its last launch: those after all sequences do
   int* status;
 };
 cudaError_t launch_cache_attention(const CUtensorMap& map, const AttentionParams& p, bool bf16, bool full, int grid,

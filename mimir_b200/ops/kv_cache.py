@@ -69,8 +69,9 @@ def cache_append(q, k, v, cos, sin, pages, scales, page_table, seq_lens, seqs, c
     ``q`` ``[tokens, heads, 128]``, ``k`` and ``v`` ``[tokens, kv_heads, 128]`` (bfloat16 or float16,
     any token and head strides that keep 16-byte alignment: slices of a packed projection are fine);
     ``cos`` and ``sin`` float32 ``[positions, 128]``, indexed by a token's position in its sequence.
-    Rows beyond ``cu_new[-1]`` give zeros.  Positions and sums are float32; q is rounded once to its type,
-    k and v once to the 8 bits.  A block that grows beyond its scale has its older tokens rounded again.
+    Rows before ``cu_new[0]`` and beyond ``cu_new[-1]`` give zeros.  Positions and sums are float32; q is rounded
+    once to its type, k and v once to the 8 bits.  A block that grows beyond its scale has its older tokens
+    rounded again.
     """
     if kernels_enabled(pages):
         return ext().cache_append(q, k, v, cos, sin, pages, scales, page_table, seq_lens, seqs, cu_new)
@@ -147,8 +148,8 @@ def cache_attention(q, pages, scales, page_table, seq_lens, seqs, cu_new, prefix
     ``q`` ``[tokens, heads, 128]`` (rotated; bfloat16 or float16); returns the same shape and type.
     A token at position ``p`` sees the positions up to ``p``; where ``p`` lies in the first
     ``prefix_lens[i]`` (int32, optional) of its sequence it sees all of those (the prefix-LM rule of
-    :func:`mimir_b200.ops.prefixlm_attention`).  A token that sees nothing, and rows beyond
-    ``cu_new[-1]``, give zeros.  ``softmax_scale`` is ``head_dim ** -0.5`` by default.
+    :func:`mimir_b200.ops.prefixlm_attention`).  A token that sees nothing, and rows before
+    ``cu_new[0]`` or beyond ``cu_new[-1]``, give zeros.  ``softmax_scale`` is ``head_dim ** -0.5`` by default.
 
     ``max_new`` (the most new tokens of one sequence, if known on the host) lets few rows take a narrower
     kernel; it changes no result beyond rounding.

@@ -564,3 +564,25 @@ def test_a_hint_below_the_real_number_of_new_tokens(heads, kv, dtype):
     for hint in (1, 2, 9):
         stale((sum(counts), heads, DIM), dtype)
         check_attention(st, list(range(6)), counts, heads, dtype, max_new=hint, kernel=1)
+
+
+@pytest.mark.parametrize("kernel", [1, 2])
+@pytest.mark.parametrize("many", [2, 40])
+def test_rows_before_the_first_sequence_are_zero(kernel, many):
+    counts = [3, 30] * (many // 2)
+    st = filled([50, 30] * (many // 2), 2, 32)
+    q = torch.randn(4 + sum(counts) + 2, 8, DIM, device=DEV).bfloat16()
+    cu = [4 + sum(counts[:i]) for i in range(many + 1)]
+    want = attend(q[4:-2], st, list(range(many)), [c - 4 for c in cu], kernel=kernel)
+    stale(q.shape, q.dtype)
+    got = attend(q, st, list(range(many)), cu, kernel=kernel)
+    check_kernel_status(DEV)
+    assert not got[:4].any() and not got[-2:].any() and torch.equal(got[4:-2], want)
+
+
+def test_append_of_rows_before_the_first_sequence():
+    st = filled([50, 30], 2, 32)
+    x = torch.randn(39, 4, DIM, device=DEV).bfloat16()
+    stale(x.shape, x.dtype)
+    got = append_both(st, x, x[:, :2], x[:, 2:], [0, 1], [4, 7, 37])
+    assert not got[:4].any() and not got[37:].any() and got[4].any()
