@@ -151,9 +151,8 @@ struct Segment {
 // Sequence i of the batch; a bad slot or length is reported and read as no tokens.
 __device__ Seq load_seq(const Params& p, int i) {
   Seq s;
-  s.row = p.cu[i];
-  s.count = max(min(p.cu[i + 1], p.tokens) - s.row, 0);
-  if (s.row < 0) s.count = 0;
+  const NewRows rows = new_rows(p.cu, i, p.tokens);
+  s.row = rows.first, s.count = rows.count;
   s.slot = p.seqs[i];
   s.prefix = p.prefix != nullptr ? p.prefix[i] : 0;
   s.len = 0;
@@ -161,8 +160,8 @@ __device__ Seq load_seq(const Params& p, int i) {
     s.slot = 0;
     if (s.count > 0) record_status(p.status, kCacheBadSlot);
   } else {
-    s.len = p.lens[s.slot];
-    if (s.len < s.count) record_status(p.status, kCacheBadLength);
+    s.len = rows.good ? p.lens[s.slot] : 0;
+    if (s.len < s.count || !rows.good) record_status(p.status, kCacheBadLength);
     if (s.len < 0) s.len = 0;
     if (s.len > p.width * p.page) {
       s.len = p.width * p.page;

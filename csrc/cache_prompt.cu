@@ -202,10 +202,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     // Blocks of the longest sequences come first, within a sequence those of its last tokens, which see most where
     // it is causal: the GPU's last blocks are then short ones (five prompts of 1343 to 4096 tokens: 416 -> 392 us).
     // Lane i has sequence i.
-    const int at = min(lane, p.n), from = p.cu[at], slot = at < p.n ? p.seqs[at] : -1;
+    const int at = min(lane, p.n), slot = at < p.n ? p.seqs[at] : -1;
     const int keys = slot >= 0 && slot < p.slots ? p.lens[slot] : 0;
-    const int news = at < p.n && from >= 0 ? max(min(p.cu[at + 1], p.tokens) - from, 0) : 0;
-    const int blocks = (news + per - 1) / per;
+    const NewRows rows = at < p.n ? new_rows(p.cu, at, p.tokens) : NewRows{0, 0, true};
+    const int blocks = (rows.count + per - 1) / per;
     int before = 0;
     for (int i = 0; i < p.n; ++i) {
       const int keys_i = __shfl_sync(0xffffffffu, keys, i), blocks_i = __shfl_sync(0xffffffffu, blocks, i);
@@ -223,15 +223,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int size = p.n + 1; size > 1;) {
       const int step = (size + 31) / 32;
       const int at = min(lo + lane * step, p.n);
-      const int c = __popc(__ballot_sync(0xffffffffu, lo + lane * step < lo + size && p.cu[at] / per + 2 * at <= b));
+      const int c = __popc(__ballot_sync(0xffffffffu, lo + lane * step < lo + size && max(p.cu[at], 0) / per + 2 * at <= b));
       const int next = lo + max(c - 1, 0) * step;
       size = min(step, lo + size - next);
       lo = next;
     }
-    tok0 = lo < p.n ? (b - (p.cu[lo] / per + 2 * lo)) * per : 0;
+    if (b == last) lo = p.n;  // as it is where the bounds are right
+    tok0 = lo < p.n ? (b - (max(p.cu[lo], 0) / per + 2 * lo)) * per : 0;
   }
   if (lo >= p.n) {
-    // rows that belong to no sequence: one block per head, which has never any of its own, clears them
+    // rows that belong to no sequence: one block per head, which has never any of its own, clears them,
+    // and one looks at the bounds
     if (blockIdx.x / p.KV == (p.n <= 32 ? last : 0)) {
       auto clear_rows = [&](int from, int to) {
         uint4* o = reinterpret_cast<uint4*>(p.out);
@@ -243,17 +245,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       if (p.first_batch) clear_rows(0, min(max(p.cu[0], 0), p.tokens));
       if (p.last_batch) clear_rows(min(max(p.cu[p.n], 0), p.tokens), p.tokens);
+      if (kvh == 0) check_bounds(p.cu, p.n, p.tokens, p.status);
     }
     return;
   }
-  const int first_row = p.cu[lo], count = first_row < 0 ? 0 : max(min(p.cu[lo + 1], p.tokens) - first_row, 0);
+  const NewRows rows = new_rows(p.cu, lo, p.tokens);
+  const int first_row = rows.first, count = rows.count;
   if (tok0 < 0 || tok0 >= count) return;  // block-uniform, before any allocation
   const int slot = p.seqs[lo], prefix = p.prefix != nullptr ? p.prefix[lo] : 0;
   int len = 0;
   if (slot < 0 || slot >= p.slots) {
     if (threadIdx.x == 0) record_status(p.status, kCacheBadSlot);
   } else {
-    len = p.lens[slot];
+    len = rows.good ? p.lens[slot] : 0;
     if (threadIdx.x == 0 && len < count) record_status(p.status, kCacheBadLength);
     if (len > p.width * p.page) {
       len = p.width * p.page;

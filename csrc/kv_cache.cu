@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) cache_append_kernel(const A
     while (size > 1) {
       const int step = (size + 31) / 32;
       const int at = min(lo + lane * step, p.n);
-      const int c = __popc(__ballot_sync(0xffffffffu, lo + lane * step < lo + size && p.cu[at] / kCacheBlock + 3 * at <= b));
+      const int c = __popc(__ballot_sync(0xffffffffu, lo + lane * step < lo + size && max(p.cu[at], 0) / kCacheBlock + 3 * at <= b));
       const int next = lo + max(c - 1, 0) * step;
       size = min(step, lo + size - next);
       lo = next;
@@ -144,11 +144,12 @@ __global__ void __launch_bounds__(kAppendThreads, 4) cache_append_kernel(const A
     if (lane == 0) {
       int rows = 0, written = 0, row = 0, pos = 0, page = -1;
       if (lo < p.n) {
-        const int first = p.cu[lo], stop = min(p.cu[lo + 1], p.tokens), slot = p.seqs[lo];
-        const int j = b - (first / kCacheBlock + 3 * lo), count = max(stop - first, 0);
+        const NewRows own = new_rows(p.cu, lo, p.tokens);
+        const int first = own.first, count = own.count, slot = p.seqs[lo];
+        const int j = b - (max(p.cu[lo], 0) / kCacheBlock + 3 * lo);
         const bool good = slot >= 0 && slot < p.slots;
-        const int start = good ? p.lens[slot] - (p.cu[lo + 1] - first) : 0;
-        if (first >= 0 && good && start >= 0) {
+        const int start = good ? p.lens[slot] - count : 0;
+        if (own.good && good && start >= 0) {
           const int64_t block = (int64_t)(start / kCacheBlock + j) * kCacheBlock;
           const int64_t from = max(block, (int64_t)start), to = min(block + kCacheBlock, (int64_t)start + count);
           rows = (int)max(to - from, (int64_t)0);
@@ -164,7 +165,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) cache_append_kernel(const A
               page = -1;
             }
           }
-        } else if (first >= 0 && j >= 0) {  // its rows become zeros
+        } else if (j >= 0) {  // its rows become zeros
           rows = min(max(count - j * kCacheBlock, 0), kCacheBlock);
           row = first + j * kCacheBlock;
           if (rows > 0) report(p.status, good ? kCacheBadLength : kCacheBadSlot);
@@ -176,13 +177,14 @@ __global__ void __launch_bounds__(kAppendThreads, 4) cache_append_kernel(const A
     (&tops[0][0])[threadIdx.x - 32] = 0;
     (&poisoned[0][0])[threadIdx.x - 32] = 0;
   }
-  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) {  // rows that belong to no sequence
+  if (blockIdx.x == gridDim.x - 1 && blockIdx.y == 0) {  // rows that belong to no sequence; all bounds
     uint4* o = reinterpret_cast<uint4*>(p.q_out);
     const int64_t per = (int64_t)p.H * kCacheDim / 8;
     const int64_t before = (p.n > 0 ? min(p.cu[0], p.tokens) : 0) * per;
     const int64_t from = (p.n > 0 ? min(max(p.cu[p.n], 0), p.tokens) : 0) * per;
     for (int64_t x = threadIdx.x; x < before; x += kAppendThreads) o[x] = make_uint4(0, 0, 0, 0);
     for (int64_t x = from + threadIdx.x; x < p.tokens * per; x += kAppendThreads) o[x] = make_uint4(0, 0, 0, 0);
+    check_bounds(p.cu, p.n, p.tokens, p.status);
   }
   __syncthreads();
   const int rows = at_rows, written = at_written, pos0 = at_pos, page = at_page;

@@ -27,7 +27,8 @@ enum CacheStatus : int {
   kCacheOk = 0,
   kCacheBadSlot = 1,    // a slot outside the page table
   kCacheBadPage = 2,    // a page that the table does not hold, or one outside the pool
-  kCacheBadLength = 3,  // fewer tokens in a slot than new ones, or a position outside the rotary tables
+  kCacheBadLength = 3,  // fewer tokens in a slot than new ones, a position outside the rotary tables, or rows
+                        // of a sequence outside the call's
   kCacheTimeout = 4,    // a wait inside a kernel ran out
 };
 
@@ -52,6 +53,24 @@ inline cudaError_t launch_after_previous(void (*kernel)(P...), dim3 grid, int th
 }
 #ifdef __CUDACC__
 __device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Rows cu[i] .. cu[i + 1] of sequence i, as far as the call has them.  Not `good` where they leave its rows or
+// run backwards: the sequence is skipped then, its rows become zeros, and kCacheBadLength is reported.  (Bounds
+// that run backwards by more than a block of rows may leave rows unwritten in the kernels that search them.)
+struct NewRows {
+  int first, count;
+  bool good;
+};
+__device__ __forceinline__ NewRows new_rows(const int* cu, int i, int tokens) {
+  const int a = cu[i], b = cu[i + 1];
+  const int first = min(max(a, 0), tokens);
+  return {first, max(min(b, tokens) - first, 0), a >= 0 && a <= b && b <= tokens};
+}
+// The report, by a block that has no rows of its own.
+__device__ __forceinline__ void check_bounds(const int* cu, int n, int tokens, int* status) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x)
+    if (!new_rows(cu, i, tokens).good) atomicCAS(status, 0, kCacheBadLength);
+}
 #endif
 
 // ---------------------------------------------------------------- kv_cache.cu

@@ -62,6 +62,12 @@ def _check_batch(page_table, seq_lens, seqs, cu_new, dev) -> None:
     _need(cu_new.shape[0] == seqs.shape[0] + 1, "cu_new needs one more entry than seqs")
 
 
+def _bounds(cu_new, rows: int) -> list[int]:
+    bounds = cu_new.tolist()
+    _need(all(0 <= a <= b <= rows for a, b in zip(bounds, bounds[1:])), f"cu_new must rise from 0 to at most {rows} rows")
+    return bounds
+
+
 # ---------------------------------------------------------------------------------- append
 def cache_append(q, k, v, cos, sin, pages, scales, page_table, seq_lens, seqs, cu_new):
     """Rotate new q and k, write k and v to the cache and return the rotated q.
@@ -106,7 +112,7 @@ def cache_append_reference(q, k, v, cos, sin, pages, scales, page_table, seq_len
           "cos and sin must be float32 tables [positions, head_dim]")
     page = pages.shape[3]
     out = torch.zeros_like(q, memory_format=torch.contiguous_format)
-    bounds, slots, lens = cu_new.tolist(), seqs.tolist(), seq_lens.tolist()
+    bounds, slots, lens = _bounds(cu_new, q.shape[0]), seqs.tolist(), seq_lens.tolist()
     for i, slot in enumerate(slots):
         first, end = bounds[i], bounds[i + 1]
         start = lens[slot] - (end - first)
@@ -185,7 +191,7 @@ def cache_attention_reference(q, pages, scales, page_table, seq_lens, seqs, cu_n
         _need(prefix_lens.shape[0] == seqs.shape[0], "prefix_lens needs one length for each of seqs")
     scale = q.shape[-1] ** -0.5 if softmax_scale is None else softmax_scale
     out = torch.zeros_like(q, memory_format=torch.contiguous_format)
-    bounds, slots = cu_new.tolist(), seqs.tolist()
+    bounds, slots = _bounds(cu_new, q.shape[0]), seqs.tolist()
     prefixes = [0] * len(slots) if prefix_lens is None else prefix_lens.tolist()
     for i, slot in enumerate(slots):
         first, end, length = bounds[i], bounds[i + 1], int(seq_lens[slot])

@@ -286,3 +286,14 @@ def test_logits_rules_one_by_one():
     assert torch.isinf(ops.process_logits(x, allowed=ints([[0]]))).all()
     y = x.clone()
     assert ops.process_logits(y, allowed=ints([[0]]), out=y) is y and torch.isinf(y).all()
+
+
+@pytest.mark.parametrize("cu", [[-1, 2], [0, 4], [2, 1]])
+def test_bounds_that_leave_the_rows_are_refused(cu):
+    st = pool(4, 2, 16, 8, 3, 2)
+    ops.cache_reserve(st["table"], st["lens"], st["refs"], [0], [20], 16)
+    x, rest = torch.randn(3, 2, 8), (st["pages"], st["scales"], st["table"], st["lens"], ints([0]), ints(cu))
+    with pytest.raises(ValueError, match="cu_new must rise"):
+        ops.cache_append(x, x, x, *tables(48, 8), *rest)
+    with pytest.raises(ValueError, match="cu_new must rise"):
+        ops.cache_attention(x, *rest)

@@ -586,3 +586,27 @@ def test_append_of_rows_before_the_first_sequence():
     stale(x.shape, x.dtype)
     got = append_both(st, x, x[:, :2], x[:, 2:], [0, 1], [4, 7, 37])
     assert not got[:4].any() and not got[37:].any() and got[4].any()
+
+
+@pytest.mark.parametrize("cu,bad", [([-3, 2, 4], [0, 1]), ([0, 2, 9], [2, 3, 4]), ([-5, -2, 3], [0, 1, 2]), ([0, 3, 1], [])])
+def test_bounds_that_leave_the_rows_are_reported(cu, bad):
+    """A sequence whose rows begin before the first or end after the last one is skipped: its rows are zeros."""
+    st = filled([60, 70], 2, 32)
+    q = torch.randn(5, 8, DIM, device=DEV).bfloat16()
+    for kernel in (1, 2):
+        stale(q.shape, q.dtype)
+        out = attend(q, st, [0, 1], cu, kernel=kernel)
+        assert torch.isfinite(out).all() and not out[bad].any()
+        assert kernel_status(DEV)["kv_cache"] == 3
+    cos, sin = (t.to(DEV) for t in tables(128, DIM))
+    before = st["pages"].clone(), st["scales"].clone()
+    stale(q.shape, q.dtype)
+    out = ops.cache_append(q, q[:, :2], q[:, :2], cos, sin, st["pages"], st["scales"], st["table"], st["lens"],
+                           ints([0, 1]).to(DEV), ints(cu).to(DEV))
+    assert torch.isfinite(out).all() and not out[bad].any()
+    assert kernel_status(DEV)["kv_cache"] == 3
+    held = [i for i in range(2) if cu[i] < 0 or cu[i + 1] > 5]  # the sequences that are skipped
+    for i in held:
+        rows = st["table"][i, :3].long()
+        rows = rows[rows >= 0]
+        assert torch.equal(st["pages"].view(torch.uint8)[rows], before[0].view(torch.uint8)[rows])
