@@ -314,15 +314,15 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
   if (threadIdx.x == 0) first[p.n] = scan_base;
   __syncthreads();
   const int64_t total = first[p.n];
-  // rows that belong to no sequence
-  auto clear_rows = [&](int64_t from, int64_t to) {
+  // Rows that belong to no sequence: a warp a block, when it has nothing else to do.
+  auto clear_rows = [&]() {
     uint4* o = reinterpret_cast<uint4*>(p.out);
-    const int64_t per = (int64_t)p.H * kCacheDim * sizeof(T) / 16;
-    for (int64_t k = from * per + blockIdx.x * (int64_t)kThreads + threadIdx.x; k < to * per; k += (int64_t)gridDim.x * kThreads)
-      o[k] = make_uint4(0, 0, 0, 0);
+    const int64_t per = (int64_t)p.H * kCacheDim * sizeof(T) / 16, step = gridDim.x * 32;
+    const int64_t before = p.first_batch ? min(p.cu[0], p.tokens) : 0;
+    const int64_t after = p.last_batch ? min(max(p.cu[p.n], 0), p.tokens) : p.tokens;
+    for (int64_t k = blockIdx.x * 32 + lane; k < before * per; k += step) o[k] = make_uint4(0, 0, 0, 0);
+    for (int64_t k = after * per + blockIdx.x * 32 + lane; k < p.tokens * per; k += step) o[k] = make_uint4(0, 0, 0, 0);
   };
-  if (p.first_batch) clear_rows(0, min(p.cu[0], p.tokens));
-  if (p.last_batch) clear_rows(min(max(p.cu[p.n], 0), p.tokens), p.tokens);
   // A unit takes about four times as long as joining a part does, and the last block of a segment joins all of its
   // parts: few long segments are shared by fewer blocks, so that units / blocks + parts / 4 is least, but by
   // kFewBlocks where there are units for them, and with whole units a block.  One sequence, 4 key/value heads, in
@@ -333,7 +333,10 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
     const uint32_t each = (uint32_t)total / (uint32_t)best;
     blocks = min(blocks, (int64_t)(((uint32_t)total + each - 1) / each));
   }
-  if (blockIdx.x >= blocks) return;
+  if (blockIdx.x >= blocks) {
+    if (warp == kWarps) clear_rows();
+    return;
+  }
   auto share = [&](int64_t b) {
     return total < (1 << 22) ? (int64_t)((uint32_t)(total * b) / (uint32_t)blocks) : total * b / blocks;
   };
@@ -424,6 +427,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
     // no copy into this block's shared memory may outlive it
     asm volatile("cp.async.wait_all;" ::: "memory");
     for (int j = max(0, it - kStages); j < it; ++j) warp_wait(&bar->full[j % kStages], (j / kStages) & 1, p.status, kCacheTimeout);
+    clear_rows();
     return;
   }
 
