@@ -270,9 +270,10 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
   uint8_t* query_base = reinterpret_cast<uint8_t*>(block_scales + kStages * 8);  // [2][kMine][kQueryLd]
   auto* bar = reinterpret_cast<Barriers<kStages>*>(query_base + 2 * kMine * kQueryLd);
   Seq* window = reinterpret_cast<Seq*>(bar + 1);                                 // [kWindow]
-  // Units before a sequence, [n + 1]: needed until the stages are
-  int64_t* first = reinterpret_cast<int64_t*>(smem);
-  static_assert(sizeof(int64_t) * (kAttentionSeqs + 1) <= kStages * kStageBytes, "the line fits the stages");
+  // Units before a sequence, [n + 1]: needed until the join buffer is.  (Not in the stages: TMA writes those, in
+  // no order with the ordinary stores of the line but by a proxy fence.)
+  int64_t* first = reinterpret_cast<int64_t*>(joined);
+  static_assert(sizeof(int64_t) * (kAttentionSeqs + 1) <= sizeof(float) * kWarps * kMine * kOutLd, "the line fits the join buffer");
   __shared__ int64_t scan_sums[kThreads / 32];
   __shared__ int64_t scan_base;
   __shared__ int last_of[2];

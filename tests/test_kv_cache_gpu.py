@@ -610,3 +610,15 @@ def test_bounds_that_leave_the_rows_are_reported(cu, bad):
         rows = st["table"][i, :3].long()
         rows = rows[rows >= 0]
         assert torch.equal(st["pages"].view(torch.uint8)[rows], before[0].view(torch.uint8)[rows])
+
+
+@pytest.mark.parametrize("many", [1, 5, 33, 160, 161, 1024, 1025, 2100])
+def test_the_line_of_sequences(many):
+    """Shares of whole units over few and many sequences, beyond one launch's too; both widths of row tiles."""
+    lens = [1 + (i * 331) % 200 for i in range(many)]
+    lens[0] = 9000 if many < 40 else 700
+    st = filled(lens, 2, 64, seed=many)
+    order = [(i * 17) % many if many % 17 else i for i in range(many)]
+    check_attention(st, order, [1] * many, 8, max_new=1, kernel=1)
+    counts = [min(lens[s], 1 + s % 6) for s in order]
+    check_attention(st, order, counts, 8, kernel=1)
