@@ -107,7 +107,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 && kRows != kRowsAlig
   }
   int b0 = 0, b1 = 0;
   if (p.bias_offsets != nullptr) {
-    b0 = max(p.bias_offsets[row], 0);
+    b0 = min(max(p.bias_offsets[row], 0), p.bias_count);  // what is added to it stays in 32 bits
     b1 = min(p.bias_offsets[row + 1], p.bias_count);
   }
   const int* ids = p.tokens + row * p.tokens_ld;

@@ -455,7 +455,7 @@ at::Tensor process_logits(at::Tensor logits, c10::optional<at::Tensor> tokens, c
   SERVING_CHECK(bias_offsets.has_value() == bias_ids.has_value() && bias_ids.has_value() == bias_values.has_value(),
                     "bias is (offsets, ids, values)");
   if (bias_ids.has_value()) {
-    SERVING_CHECK(bias_ids->size(0) < (int64_t(1) << 31) - 64, "too many biases");
+    SERVING_CHECK(bias_ids->dim() == 1 && bias_ids->size(0) < (int64_t(1) << 31) - 1024, "too many biases");
     per_row(given(bias_ids), "the bias ids", at::kInt, bias_ids->numel());
     per_row(given(bias_values), "the bias values", at::kFloat, bias_ids->numel());
   }

@@ -24,7 +24,7 @@ def process_logits(logits, *, tokens=None, token_lens=None, prompt_lens=None, re
     * the frequency and presence penalties: ``- frequency[row] * c - presence[row]`` for a token that was
       generated ``c > 0`` times (tokens from ``prompt_lens[row]`` on);
     * ``bias = (offsets, ids, values)``: row ``r`` adds ``values[i]`` to token ``ids[i]`` for ``i`` in
-      ``offsets[r]:offsets[r + 1]`` (equal ids add up);
+      ``offsets[r]:offsets[r + 1]`` (equal ids add up; offsets outside the list end at its ends);
     * the mask: -inf where bit ``v % 32`` of word ``v // 32`` of ``allowed[row]`` (int32) is zero, whatever
       the logit was.  A row that allows nothing is all -inf.
 
@@ -74,7 +74,7 @@ def process_logits_reference(logits, tokens, token_lens, prompt_lens, repetition
             if presence is not None:
                 row[seen] -= presence[r]
         if offsets is not None:
-            span = slice(int(offsets[r]), int(offsets[r + 1]))
+            span = slice(max(int(offsets[r]), 0), max(int(offsets[r + 1]), 0))
             ok = (ids[span] >= 0) & (ids[span] < vocab)
             row += torch.zeros_like(row).index_add_(0, ids[span][ok].long(), values[span][ok])
     if allowed is not None:

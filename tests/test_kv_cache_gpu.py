@@ -622,3 +622,17 @@ def test_the_line_of_sequences(many):
     check_attention(st, order, [1] * many, 8, max_new=1, kernel=1)
     counts = [min(lens[s], 1 + s % 6) for s in order]
     check_attention(st, order, counts, 8, kernel=1)
+
+
+@pytest.mark.parametrize("offsets", [[2 ** 31 - 1, 2 ** 31 - 1, 2], [-5, 2, 2 ** 31 - 1], [2 ** 31 - 300, 0, -2 ** 31], [3, 2, 1]])
+def test_bias_offsets_outside_the_list(offsets):
+    x = torch.randn(2, 100, device=DEV)
+    ids, values = ints([4, 4, 9]).to(DEV), torch.tensor([1.0, 2.0, 5.0], device=DEV)
+    want = x.clone()
+    for row in range(2):
+        for i in range(max(offsets[row], 0), min(offsets[row + 1], 3)):
+            want[row, ids[i].item()] += values[i]
+    got = ops.process_logits(x, bias=(ints(offsets).to(DEV), ids, values))
+    torch.testing.assert_close(got, want, rtol=0, atol=3 * 2.0 ** -24 * 2.0 ** 4)  # three sums under 2^4
+    host = ops.process_logits(x.cpu(), bias=(ints(offsets), ids.cpu(), values.cpu()))
+    torch.testing.assert_close(host, want.cpu(), rtol=0, atol=3 * 2.0 ** -24 * 2.0 ** 4)
