@@ -513,7 +513,8 @@ __global__ void __launch_bounds__(kBook) cache_fork_kernel(const Book b, const i
       report(b.status, kCacheBadSlot);
       last = -2;
     } else {
-      const int len = b.lens[s], whole = len / b.page;
+      if (b.lens[s] < 0) report(b.status, kCacheBadLength);  // read as none
+      const int len = max(b.lens[s], 0), whole = len / b.page;
       if (len % b.page != 0) {
         last = whole < b.width ? b.table[(int64_t)s * b.width + whole] : -1;
         if (last < 0 || last >= b.npages) {
@@ -527,7 +528,7 @@ __global__ void __launch_bounds__(kBook) cache_fork_kernel(const Book b, const i
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kBook)  // after every source length has been read
-    if (from[i] != -2) b.lens[dst[i]] = b.lens[src[i]];
+    if (from[i] != -2) b.lens[dst[i]] = max(b.lens[src[i]], 0);
   const int total = scan_needs(need, n, warp_sums);
   const int have = find_free(b.refs, b.npages, min(total, b.npages), found, warp_sums);
   const bool ok = have >= total;

@@ -636,3 +636,22 @@ def test_bias_offsets_outside_the_list(offsets):
     torch.testing.assert_close(got, want, rtol=0, atol=3 * 2.0 ** -24 * 2.0 ** 4)  # three sums under 2^4
     host = ops.process_logits(x.cpu(), bias=(ints(offsets), ids.cpu(), values.cpu()))
     torch.testing.assert_close(host, want.cpu(), rtol=0, atol=3 * 2.0 ** -24 * 2.0 ** 4)
+
+
+def test_forks_of_a_negative_length():
+    """Reported, read as no tokens: nothing outside the table is looked at."""
+    st = {k: t.to(DEV) for k, t in pool(8, 1, 16, DIM, 3, 4, layers=2).items()}
+    book = (st["table"], st["lens"], st["refs"])
+    ops.cache_reserve(*book, [0, 1, 2], [20, 40, 17], 16)
+    st["lens"][0] = -20
+    before = [t.clone() for t in (st["pages"].view(torch.uint8), st["scales"])]
+    held = st["table"][:2].clone()
+    assert ops.cache_fork(st["pages"], st["scales"], *book, [0, 1], [3, 2]).item() == 0
+    assert kernel_status(DEV)["kv_cache"] == 3
+    assert st["lens"].tolist() == [-20, 40, 40, 0] and st["table"][3].tolist() == [-1] * 3
+    assert torch.equal(st["table"][:2], held) and torch.equal(st["table"][2, :2], held[1, :2])
+    assert st["refs"].sum().item() == 2 + 3 + 3
+    fresh = st["table"][2, 2].long()
+    assert torch.equal(st["pages"].view(torch.uint8)[:, fresh], before[0][:, held[1, 2].long()])
+    keep = torch.arange(8, device=DEV) != fresh
+    assert torch.equal(st["pages"].view(torch.uint8)[:, keep], before[0][:, keep]) and torch.equal(st["scales"][:, keep], before[1][:, keep])
