@@ -409,9 +409,10 @@ __global__ void __launch_bounds__(kBook) cache_reserve_kernel(int* table, int sl
                                                               int page, int* found, int* missing) {
   __shared__ int need[kMaxBatch];
   __shared__ int warp_sums[32];
-  __shared__ int bad;
+  __shared__ int bad, large;
+  __shared__ int64_t sum;
   after_previous();
-  if (threadIdx.x == 0) bad = 0;
+  if (threadIdx.x == 0) bad = large = 0;
   __syncthreads();
   for (int i = threadIdx.x; i < n; i += kBook) {
     const int slot = seqs[i], c = counts[i];
@@ -425,11 +426,24 @@ __global__ void __launch_bounds__(kBook) cache_reserve_kernel(int* table, int sl
       else pages = (int)to - (len + page - 1) / page;
     }
     need[i] = pages;
+    if (pages >= (int)((int64_t(1) << 31) / kMaxBatch)) large = 1;
   }
   __syncthreads();
   if (bad) {
     if (threadIdx.x == 0) *missing = -1;
     return;
+  }
+  if (large) {  // the sum may pass 32 bits: more than the pool has then
+    if (threadIdx.x == 0) {
+      sum = 0;
+      for (int i = 0; i < n; ++i) sum += need[i];
+    }
+    __syncthreads();
+    if (sum > npages) {
+      const int have = find_free(refs, npages, npages, found, warp_sums);
+      if (threadIdx.x == 0) *missing = (int)min(sum - have, (int64_t)0x7fffffff);
+      return;
+    }
   }
   const int total = scan_needs(need, n, warp_sums);
   const int have = find_free(refs, npages, min(total, npages), found, warp_sums);

@@ -655,3 +655,14 @@ def test_forks_of_a_negative_length():
     assert torch.equal(st["pages"].view(torch.uint8)[:, fresh], before[0][:, held[1, 2].long()])
     keep = torch.arange(8, device=DEV) != fresh
     assert torch.equal(st["pages"].view(torch.uint8)[:, keep], before[0][:, keep]) and torch.equal(st["scales"][:, keep], before[1][:, keep])
+
+
+@pytest.mark.parametrize("slots,each", [(4096, 600000), (4000, 600000), (2, 524288), (1, 524287)])
+def test_reserving_more_pages_than_32_bits_count(slots, each):
+    """The sum of a batch's needs may pass 2^31 and 2^32: they lack then, and nothing changes."""
+    table = torch.full((slots, 600000), -1, dtype=torch.int32, device=DEV)
+    lens, refs = torch.zeros(slots, dtype=torch.int32, device=DEV), torch.zeros(100, dtype=torch.int32, device=DEV)
+    refs[::4] = 1
+    lack = ops.cache_reserve(table, lens, refs, list(range(slots)), [each * 16] * slots, 16).item()
+    assert lack == min(slots * each - 75, 2 ** 31 - 1)
+    assert not lens.any() and refs.sum().item() == 25 and (table[0] == -1).all() and (table[-1] == -1).all()
