@@ -639,7 +639,7 @@ __device__ __forceinline__ bool copy_item(const CopyParams& p, int i, int& a, in
   return !(a == b && p.pages == p.out_pages);
 }
 
-// blockIdx.y: layer; blockIdx.x: a share of the list.
+// blockIdx.y: layers y, y + gridDim.y, ...; blockIdx.x: a share of the list.
 __global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const CopyParams p) {
   after_previous();
   if (p.missing != nullptr && *p.missing != 0) return;
@@ -647,20 +647,22 @@ __global__ void __launch_bounds__(kCopyThreads) cache_copy_kernel(const CopyPara
   for (int i = blockIdx.x; i < p.n; i += gridDim.x) {
     int a, b;
     if (!copy_item(p, i, a, b)) continue;
-    const int64_t in = blockIdx.y * p.npages + a, out = blockIdx.y * p.out_npages + b;
-    const uint4* s = reinterpret_cast<const uint4*>(p.pages + in * p.page_bytes);
-    uint4* o = reinterpret_cast<uint4*>(p.out_pages + out * p.page_bytes);
-    for (int first = threadIdx.x; first < end; first += kCopyThreads * kCopyAhead) {
-      uint4 v[kCopyAhead];
+    for (int layer = blockIdx.y; layer < p.layers; layer += gridDim.y) {
+      const int64_t in = layer * p.npages + a, out = layer * p.out_npages + b;
+      const uint4* s = reinterpret_cast<const uint4*>(p.pages + in * p.page_bytes);
+      uint4* o = reinterpret_cast<uint4*>(p.out_pages + out * p.page_bytes);
+      for (int first = threadIdx.x; first < end; first += kCopyThreads * kCopyAhead) {
+        uint4 v[kCopyAhead];
 #pragma unroll
-      for (int u = 0; u < kCopyAhead; ++u)
-        if (first + u * kCopyThreads < end) v[u] = __ldcs(s + first + u * kCopyThreads);
+        for (int u = 0; u < kCopyAhead; ++u)
+          if (first + u * kCopyThreads < end) v[u] = __ldcs(s + first + u * kCopyThreads);
 #pragma unroll
-      for (int u = 0; u < kCopyAhead; ++u)
-        if (first + u * kCopyThreads < end) __stcs(o + first + u * kCopyThreads, v[u]);
+        for (int u = 0; u < kCopyAhead; ++u)
+          if (first + u * kCopyThreads < end) __stcs(o + first + u * kCopyThreads, v[u]);
+      }
+      for (int f = threadIdx.x; f < p.scale_floats; f += kCopyThreads)
+        p.out_scales[out * p.scale_floats + f] = p.scales[in * p.scale_floats + f];
     }
-    for (int f = threadIdx.x; f < p.scale_floats; f += kCopyThreads)
-      p.out_scales[out * p.scale_floats + f] = p.scales[in * p.scale_floats + f];
   }
   if (p.out_table != nullptr) {
     const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x, blocks = (int64_t)gridDim.x * gridDim.y;

@@ -666,3 +666,13 @@ def test_reserving_more_pages_than_32_bits_count(slots, each):
     lack = ops.cache_reserve(table, lens, refs, list(range(slots)), [each * 16] * slots, 16).item()
     assert lack == min(slots * each - 75, 2 ** 31 - 1)
     assert not lens.any() and refs.sum().item() == 25 and (table[0] == -1).all() and (table[-1] == -1).all()
+
+
+def test_copies_of_more_layers_than_a_grid_has_rows():
+    layers = 65535 + 3
+    pages = torch.zeros(layers, 2, 2, 1, 16, DIM, dtype=torch.uint8, device=DEV)
+    pages[:, 0] = torch.arange(layers, device=DEV).remainder(120).to(torch.uint8)[:, None, None, None, None]
+    scales = torch.arange(layers, device=DEV, dtype=torch.float32)[:, None, None, None, None].repeat(1, 2, 2, 1, 1)
+    scales[:, 1] = 0
+    ops.cache_copy(pages.view(torch.float8_e4m3fn), scales, ints([0]).to(DEV), ints([1]).to(DEV))
+    assert torch.equal(pages[:, 1], pages[:, 0]) and torch.equal(scales[:, 1], scales[:, 0])
