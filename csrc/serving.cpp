@@ -1,6 +1,7 @@
 // The serving operators' entry points: checks of the tensors, workspaces, launches on the current stream.
 // Device code and layouts: serving.h.
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -135,9 +136,10 @@ CUtensorMap queries_map(const at::Tensor& q, int64_t group) {
   return map;
 }
 
-// Counters that are zero before and after every call, and room for partial sums.  Both are kept per stream, whose
-// calls follow one another.  A graph may run beside the stream that it was captured on: it has counters of
+// Counters that are zero before and after every call, and room for partial sums (7.4 MB).  Both are kept per stream,
+// whose calls follow one another.  A graph may run beside the stream that it was captured on: it has counters of
 // its own (per stream of the capture, cleared at its first call), and its partial sums come from its pool.
+// Its counters do not: they outlive it, and would hold a whole segment of that pool.
 struct AttentionParts {
   float2 ml[kAttentionBlocks][2][kAttentionRows];
   float sums[kAttentionBlocks][2][kAttentionRows][kCacheDim];
@@ -159,7 +161,19 @@ AttentionWork attention_work(const at::Device& dev, cudaStream_t stream) {
   std::lock_guard<std::mutex> lock(mutex);
   AttentionWork& work = (*kept)[{dev.index(), stream, capture}];
   if (!work.arrived.defined()) {
-    work.arrived = at::empty({kAttentionBlocks * (int64_t)sizeof(int)}, bytes);
+    {
+      c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+      // Memory asked for on a stream that is not captured is the common pool's; always the same stream, since
+      // every stream has segments of its own.
+      static std::map<int, c10::cuda::CUDAStream> others;
+      c10::cuda::OptionalCUDAStreamGuard other;
+      if (capture != 0) {
+        auto it = others.find(dev.index());
+        if (it == others.end()) it = others.emplace(dev.index(), c10::cuda::getStreamFromPool(false, dev.index())).first;
+        other.reset_stream(it->second);
+      }
+      work.arrived = at::empty({kAttentionBlocks * (int64_t)sizeof(int)}, bytes);
+    }
     C10_CUDA_CHECK(cudaMemsetAsync(work.arrived.data_ptr(), 0, kAttentionBlocks * sizeof(int), stream));
     if (capture == 0) work.parts = at::empty({(int64_t)sizeof(AttentionParts)}, bytes);
   }

@@ -676,3 +676,31 @@ def test_copies_of_more_layers_than_a_grid_has_rows():
     scales[:, 1] = 0
     ops.cache_copy(pages.view(torch.float8_e4m3fn), scales, ints([0]).to(DEV), ints([1]).to(DEV))
     assert torch.equal(pages[:, 1], pages[:, 0]) and torch.equal(scales[:, 1], scales[:, 0])
+
+
+def test_graphs_leave_little_memory_behind():
+    """Counters that outlive a graph do not come from its own pool, of which each would hold a segment."""
+    st = filled([600, 130], 2, 64)
+    q = torch.randn(2, 8, DIM, device=DEV).bfloat16()
+    args = (st["pages"], st["scales"], st["table"], st["lens"], ints([0, 1]).to(DEV), ints([0, 1, 2]).to(DEV))
+    want = ops.cache_attention(q, *args)
+
+    def capture():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.cache_attention(q, *args)
+            again = ops.cache_attention(out, *args)
+        for _ in range(2):
+            graph.replay()
+            assert torch.equal(out, want) and torch.equal(again, ops.cache_attention(want, *args))
+        graph.reset()
+
+    capture()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_reserved()
+    for _ in range(6):
+        capture()
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    assert torch.cuda.memory_reserved() - before <= 2 * 2 ** 20
