@@ -128,6 +128,10 @@ class Batch:
                                    max_new=self.max_new)
 
 
+FLOAT32_MAX = torch.finfo(torch.float32).max
+LEAST_TEMPERATURE = 1e-30  # logits divided by it stay in float32
+
+
 @dataclass
 class Request:
     """One prompt and its decoding rule (OpenAI's fields; ``repetition_penalty`` as Transformers has it)."""
@@ -150,8 +154,21 @@ class Request:
             raise ValueError(f"a prompt of {len(self.ids)} tokens does not fit {max_len} positions")
         if self.n < 1 or self.max_tokens < 1 or self.repetition_penalty <= 0:
             raise ValueError("n, max_tokens and repetition_penalty must be positive")
+        # (comparisons that NaN does not pass)
+        if not -FLOAT32_MAX <= self.temperature <= FLOAT32_MAX or 0 < self.temperature < LEAST_TEMPERATURE:
+            raise ValueError(f"temperature must be zero (greedy) or at least {LEAST_TEMPERATURE}, and finite")
+        if not self.top_p > 0:
+            raise ValueError("top_p must be positive")
+        if not 2.0 ** -126 <= self.repetition_penalty <= 2.0 ** 126:
+            raise ValueError("repetition_penalty and its inverse must be float32 numbers")
+        if not all(abs(x) <= FLOAT32_MAX for x in (self.presence_penalty, self.frequency_penalty)):
+            raise ValueError("presence_penalty and frequency_penalty must be finite float32 numbers")
         if any(not 0 <= int(i) < vocab for i in self.logit_bias):
             raise ValueError("logit_bias names tokens of the vocabulary")
+        if any(not v <= FLOAT32_MAX for v in self.logit_bias.values()):
+            raise ValueError("logit_bias holds finite float32 numbers, or -inf")
+        if self.seed is not None and not -2 ** 63 <= self.seed <= 2 ** 64 - self.n:
+            raise ValueError("seed must lie in 64 bits, with one for each of the n completions")
         if self.allowed_token_ids is not None and not any(0 <= int(i) < vocab for i in self.allowed_token_ids):
             raise ValueError("allowed_token_ids allows no token of the vocabulary")
 

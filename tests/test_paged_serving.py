@@ -244,3 +244,52 @@ def test_refusals_on_the_gpu(tmp_path):
         PagedDecoder(_model(tmp_path / "a", {}, "cuda", torch.bfloat16))
     with pytest.raises(ValueError, match="bfloat16 or float16"):
         PagedDecoder(_model(tmp_path / "b", GPU, "cuda", torch.float32))
+
+
+# ---------------------------------------------------------------------------------- requests that cannot be served
+BAD_VALUES = [dict(temperature=float("nan")), dict(temperature=float("inf")), dict(temperature=1e-40),
+              dict(temperature=1.0, top_p=-1.0), dict(temperature=1.0, top_p=0.0), dict(top_p=float("nan")),
+              dict(repetition_penalty=1e-40), dict(repetition_penalty=1e39), dict(repetition_penalty=float("nan")),
+              dict(presence_penalty=float("nan")), dict(presence_penalty=1e39), dict(frequency_penalty=float("-inf")),
+              dict(logit_bias={5: float("nan")}), dict(logit_bias={5: 1e39}), dict(temperature=1.0, seed=2 ** 70),
+              dict(temperature=1.0, seed=2 ** 64 - 1, n=2), dict(temperature=1.0, seed=-2 ** 63 - 1)]
+
+
+@pytest.mark.parametrize("bad", BAD_VALUES, ids=str)
+def test_values_that_would_fail_in_the_batch_are_refused(bad):
+    with pytest.raises(ValueError):
+        Request([1, 2], **bad).check(96, 64)
+
+
+@pytest.mark.parametrize("good", [dict(temperature=-1.0), dict(temperature=1e-30), dict(temperature=1.0, top_p=5.0),
+                                  dict(temperature=1.0, top_p=1e-30), dict(repetition_penalty=2.0 ** -126),
+                                  dict(temperature=1.0, seed=2 ** 64 - 1), dict(temperature=1.0, seed=-2 ** 63),
+                                  dict(logit_bias={5: float("-inf")}, temperature=0.7), dict(presence_penalty=3e38)], ids=str)
+def test_values_at_the_edges_are_served(tmp_path, good):
+    dec = PagedDecoder(_model(tmp_path), slots=4)
+    assert len(dec.generate([Request([1, 2], max_tokens=4, **good)])[0][0]) == 4
+
+
+def test_bad_requests_do_not_reach_the_batch(tmp_path):
+    from test_transformers_model import _export
+    _export(tmp_path, {})
+    engine, server, url = _serve(tmp_path, "cpu")
+    try:
+        good = {"prompt": "w1 w2", "max_tokens": 4}
+        want = json.loads(_post(url, good)[1])["choices"]
+        bodies = [good, {"prompt": "w3", "temperature": 1.0, "top_p": -1}, {"prompt": "w3", "temperature": 1e-39},
+                  {"prompt": "w3", "temperature": 1, "seed": 2 ** 70}]
+        got = [None] * len(bodies)
+
+        def ask(i):
+            got[i] = _post(url, bodies[i])
+
+        threads = [threading.Thread(target=ask, args=(i,)) for i in range(len(bodies))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(timeout=120)
+        assert json.loads(got[0][1])["choices"] == want and [g[0] for g in got[1:]] == [400] * 3
+    finally:
+        server.shutdown()
+        server.server_close()
