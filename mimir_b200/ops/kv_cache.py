@@ -32,6 +32,7 @@ from mimir_b200.ops._ext import ext, kernels_enabled
 BLOCK = 16       # tokens that share a scale
 MIN_EXPONENT = -32
 PAGE_SIZES = (16, 32, 64, 128, 256)
+MAX_SEQUENCES = 4096  # of one cache_reserve or cache_fork on CUDA
 
 
 def _need(condition: bool, message: str) -> None:

@@ -26,7 +26,7 @@ at a time.
 
 ``--kv-cache fp8`` decodes over the 8-bit paged cache instead (:mod:`mimir_b200.serving.paged`; on CUDA a
 bfloat16 or float16 model with heads of 128): half the memory of a 16-bit cache and no padding, so that
-requests of any decoding rule and any seed share a batch, and the further fields ``n`` (completions that share
+requests of any decoding rule and any seed share a batch, and the further fields ``n`` (up to 128 completions that share
 the prompt's pages), ``presence_penalty``, ``frequency_penalty``, ``repetition_penalty``, ``logit_bias`` and
 ``allowed_token_ids``.
 
@@ -50,8 +50,8 @@ import torch
 class _Pending:
     """One queued greedy request and, once its batch ran, its result (or the batch's error)."""
 
-    def __init__(self, ids: list[int], body: dict):
-        self.ids, self.body = ids, body
+    def __init__(self, ids: list[int], body: dict, completions: int = 1):
+        self.ids, self.body, self.completions = ids, body, completions
         self.done = threading.Event()
         self.result = None
         self.error: Optional[BaseException] = None
@@ -156,10 +156,11 @@ class Engine:
     @torch.no_grad()
     def complete(self, ids: list[int], body: dict):
         """One result, or a list of them where a request over the paged cache asks for ``n > 1``."""
+        completions = 1
         if self.paged is not None:
-            self._request(ids, body)  # a bad request fails by itself, not with the batch it would be in
+            completions = self._request(ids, body).n  # a bad request fails by itself, not with the batch it would be in
         if self.batchable(body):
-            item = _Pending(ids, body)
+            item = _Pending(ids, body, completions)
             with self._ready:
                 self._queue.append(item)
                 self._ready.notify()
@@ -251,6 +252,19 @@ class Engine:
             sent = text
         yield None, (sent, n_in, n_out, "stop" if stopped else finish)
 
+    def _fitting(self, items: list[_Pending]) -> list[_Pending]:
+        """The first items whose completions fit a batch over the paged cache; the others wait for the next one."""
+        if self.paged is None:
+            return items
+        from mimir_b200.serving.paged import MAX_COMPLETIONS
+        total, count = 0, 0
+        for item in items:
+            total += item.completions
+            if total > MAX_COMPLETIONS:
+                break
+            count += 1
+        return items[:count]
+
     # ------------------------------------------------------------------ batched greedy decoding
     def _serve_batches(self) -> None:
         while True:
@@ -265,7 +279,7 @@ class Engine:
                 deadline = time.monotonic() + self.batch_wait
                 while len(same()) < self.max_batch and time.monotonic() < deadline:
                     self._ready.wait(max(0.0, deadline - time.monotonic()))
-                batch = same()
+                batch = self._fitting(same())
                 taken = {id(item) for item in batch}
                 self._queue = [item for item in self._queue if id(item) not in taken]
             try:

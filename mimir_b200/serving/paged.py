@@ -21,7 +21,7 @@ from typing import Iterator, Optional
 import torch
 
 from mimir_b200 import ops
-from mimir_b200.ops.kv_cache import BLOCK
+from mimir_b200.ops.kv_cache import BLOCK, MAX_SEQUENCES
 
 
 def rotary_tables(positions: int, dim: int, theta: float, device) -> tuple[torch.Tensor, torch.Tensor]:
@@ -130,6 +130,7 @@ class Batch:
 
 FLOAT32_MAX = torch.finfo(torch.float32).max
 LEAST_TEMPERATURE = 1e-30  # logits divided by it stay in float32
+MAX_COMPLETIONS = 128      # of one request, and of a server's batch: each takes a slot of the cache
 
 
 @dataclass
@@ -154,6 +155,8 @@ class Request:
             raise ValueError(f"a prompt of {len(self.ids)} tokens does not fit {max_len} positions")
         if self.n < 1 or self.max_tokens < 1 or self.repetition_penalty <= 0:
             raise ValueError("n, max_tokens and repetition_penalty must be positive")
+        if self.n > MAX_COMPLETIONS:
+            raise ValueError(f"n is at most {MAX_COMPLETIONS}")
         # (comparisons that NaN does not pass)
         if not -FLOAT32_MAX <= self.temperature <= FLOAT32_MAX or 0 < self.temperature < LEAST_TEMPERATURE:
             raise ValueError(f"temperature must be zero (greedy) or at least {LEAST_TEMPERATURE}, and finite")
@@ -251,6 +254,8 @@ class PagedDecoder:
         for r in requests:
             r.check(vocab, limit)
         slots = sum(r.n for r in requests)
+        if slots > MAX_SEQUENCES:
+            raise ValueError(f"{slots} completions side by side are more than {MAX_SEQUENCES}")
         if slots > self.cache.page_table.shape[0]:
             self._make(slots)
         cache, used = self.cache, list(range(slots))

@@ -293,3 +293,34 @@ def test_bad_requests_do_not_reach_the_batch(tmp_path):
     finally:
         server.shutdown()
         server.server_close()
+
+
+def test_completions_are_bounded(tmp_path):
+    """``n`` sizes slots, history and pool: one request has at most 128, and a batch of the server too."""
+    with pytest.raises(ValueError, match="at most 128"):
+        Request([1], n=129).check(96, 64)
+    Request([1], n=128).check(96, 64)
+    from test_transformers_model import _export
+    _export(tmp_path, {})
+    engine, server, url = _serve(tmp_path, "cpu")
+    sizes, generate = [], engine.paged.generate
+    engine.paged.generate = lambda requests, *a, **kw: sizes.append([r.n for r in requests]) or generate(requests, *a, **kw)
+    try:
+        assert _post(url, {"prompt": "w1", "n": 5000})[0] == 400
+        threads = [threading.Thread(target=_post, args=(url, {"prompt": f"w{n}", "max_tokens": 1, "n": n})) for n in (60, 60, 60, 128)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(timeout=120)
+        assert sorted(sum(sizes, [])) == [60, 60, 60, 128] and max(map(sum, sizes)) <= 128
+        assert engine.paged.cache.page_table.shape[0] <= 128
+    finally:
+        server.shutdown()
+        server.server_close()
+
+
+def test_more_completions_than_a_call_of_the_page_operations_takes(tmp_path):
+    dec = PagedDecoder(_model(tmp_path), slots=1)
+    with pytest.raises(ValueError, match="4096"):
+        dec.generate([Request([1], n=128)] * 33)
+    assert dec.cache.page_table.shape[0] == 1
