@@ -26,9 +26,9 @@ at a time.
 
 ``--kv-cache fp8`` decodes over the 8-bit paged cache instead (:mod:`mimir_b200.serving.paged`; on CUDA a
 bfloat16 or float16 model with heads of 128): half the memory of a 16-bit cache and no padding, so that
-requests of any decoding rule and any seed share a batch, and the further fields ``n`` (up to 128 completions that share
-the prompt's pages), ``presence_penalty``, ``frequency_penalty``, ``repetition_penalty``, ``logit_bias`` and
-``allowed_token_ids``.
+requests of any decoding rule and any seed share a batch, and the further fields ``n`` (up to 128
+completions that share the prompt's pages), ``presence_penalty``, ``frequency_penalty``,
+``repetition_penalty``, ``logit_bias`` and ``allowed_token_ids``.
 
 Usage: ``python -m mimir_b200.serving.native MODEL_DIR [--port 8000] [--device cuda:0]
 [--max-batch 8] [--batch-wait-ms 5] [--kv-cache model|fp8]``.
@@ -169,7 +169,10 @@ class Engine:
                 raise item.error
             return item.result
         if self.paged is not None:
-            return self._generate_batch([_Pending(ids, body)])[0]
+            result = self._generate_batch([_Pending(ids, body)])[0]
+            if isinstance(result, Exception):
+                raise result
+            return result
         temperature = float(body.get("temperature") or 0.0)
         gen = self._gen_args(self._max_tokens(body)) | dict(do_sample=temperature > 0)
         if temperature > 0:
@@ -284,6 +287,8 @@ class Engine:
                 self._queue = [item for item in self._queue if id(item) not in taken]
             try:
                 for item, result in zip(batch, self._generate_batch(batch)):
+                    if isinstance(result, Exception):  # this request's own
+                        item.error = result
                     item.result = result
             except BaseException as exc:  # the requests of a failed batch all report it
                 for item in batch:
@@ -296,9 +301,11 @@ class Engine:
     def _generate_batch(self, batch: list[_Pending]) -> list:
         if self.paged is not None:
             with self.lock:
-                out = self.paged.generate([self._request(item.ids, item.body) for item in batch], self.tokenizer.eos_token_id)
+                failed: dict = {}
+                out = self.paged.generate([self._request(item.ids, item.body) for item in batch],
+                                          self.tokenizer.eos_token_id, failed)
             results = [[self._finish(item.ids, new, item.body) for new in each] for item, each in zip(batch, out)]
-            return [r if len(r) > 1 else r[0] for r in results]
+            return [failed.get(i, r if len(r) > 1 else r[0]) for i, r in enumerate(results)]
         width = max(len(item.ids) for item in batch)
         x = torch.full((len(batch), width), self.pad_id, dtype=torch.long)
         mask = torch.zeros_like(x)

@@ -228,27 +228,37 @@ class PagedDecoder:
         return kw
 
     @staticmethod
-    def _sample(logits: torch.Tensor, rows: list[tuple[Request, int]], generators: dict) -> list[int]:
-        if all(r.temperature <= 0 for r, _ in rows):
-            return logits.argmax(-1).tolist()
-        out = []
-        for i, (r, which) in enumerate(rows):
-            row = logits[i]
+    def _sample(logits: torch.Tensor, rows: list[tuple[Request, int]], generators: dict) -> list[Optional[int]]:
+        """A token of each row; None where there is none to choose: NaN among the logits, or everything forbidden.
+        (Such rows do not come to ``torch.multinomial``, which reports them by an assertion on the device.)"""
+        best, good = logits.argmax(-1), logits.amax(-1) > -math.inf  # a maximum among NaN is NaN
+        chances = {}
+        for i, (r, _) in enumerate(rows):
             if r.temperature <= 0:
-                out.append(int(row.argmax()))
                 continue
-            p = torch.softmax(row / r.temperature, -1)
+            p = torch.softmax(logits[i] / r.temperature, -1)
             if r.top_p < 1.0:
                 order = p.argsort(descending=True, stable=True)
                 ahead = p[order].cumsum(-1) - p[order]
                 p = p.index_fill(0, order[ahead >= r.top_p], 0.0)
-            out.append(int(torch.multinomial(p, 1, generator=generators.get((id(r), which)))))
+            chances[i] = p
+        if chances:
+            sums = torch.stack([p.sum() for p in chances.values()])
+            good[list(chances)] &= (sums > 0) & (sums < math.inf)
+        out = []
+        for i, (token, ok) in enumerate(torch.stack((best, good.long()), -1).tolist()):  # one wait
+            if ok and i in chances:
+                r, which = rows[i]
+                token = int(torch.multinomial(chances[i], 1, generator=generators.get((id(r), which))))
+            out.append(token if ok else None)
         return out
 
     @torch.no_grad()
-    def run(self, requests: list[Request], eos: Optional[int] = None) -> Iterator[tuple[int, int, int]]:
+    def run(self, requests: list[Request], eos: Optional[int] = None,
+            failed: Optional[dict] = None) -> Iterator[tuple[int, int, int]]:
         """Yields ``(request, completion, token)`` as tokens are generated (the end token included), all
-        completions of all requests side by side."""
+        completions of all requests side by side.  A request that has no token to choose leaves the batch with an
+        exception, which ``failed`` takes at its number; without ``failed`` it is raised."""
         vocab = self.config.vocab_size
         limit = min(self.config.max_position_embeddings, self.history.shape[1])
         for r in requests:
@@ -289,8 +299,21 @@ class PagedDecoder:
                     kw["token_lens"] = cache.seq_lens[where]
                     kw["tokens"] = self.history[where, :max(len(r.ids) + made[k] for (r, _), k in zip(rows, live))]
                 tokens = self._sample(ops.process_logits(logits, **kw), rows, generators)
+                lost = {}
+                for row, ((i, _), token) in enumerate(zip(live, tokens)):
+                    if token is None and not bool(torch.isfinite(logits[row]).all()):
+                        lost[i] = RuntimeError("the model's logits are not finite")
+                    elif token is None:
+                        lost.setdefault(i, ValueError("the rules of the request leave no token to choose"))
+                if lost and failed is None:
+                    raise next(iter(lost.values()))
+                if lost:
+                    failed.update(lost)
                 still, ended = [], []
                 for key, token in zip(live, tokens):
+                    if key[0] in lost:
+                        ended.append((key, None))
+                        continue
                     made[key] += 1
                     yield key[0], key[1], token
                     r = requests[key[0]]
@@ -315,9 +338,10 @@ class PagedDecoder:
             if used:
                 cache.free(used)
 
-    def generate(self, requests: list[Request], eos: Optional[int] = None) -> list[list[list[int]]]:
-        """Generated tokens of every completion of every request."""
+    def generate(self, requests: list[Request], eos: Optional[int] = None,
+                 failed: Optional[dict] = None) -> list[list[list[int]]]:
+        """Generated tokens of every completion of every request (``failed`` as :meth:`run` has it)."""
         out = [[[] for _ in range(r.n)] for r in requests]
-        for i, w, token in self.run(requests, eos):
+        for i, w, token in self.run(requests, eos, failed):
             out[i][w].append(token)
         return out

@@ -324,3 +324,54 @@ def test_more_completions_than_a_call_of_the_page_operations_takes(tmp_path):
     with pytest.raises(ValueError, match="4096"):
         dec.generate([Request([1], n=128)] * 33)
     assert dec.cache.page_table.shape[0] == 1
+
+
+@pytest.mark.parametrize("rule", [dict(temperature=0.9, seed=1), dict()], ids=["sampled", "greedy"])
+def test_a_request_without_a_token_to_choose_fails_alone(tmp_path, rule):
+    """Rules that leave nothing, and logits that a poisoned cache block made NaN: that request fails, the others
+    get what they get alone."""
+    dec = PagedDecoder(_model(tmp_path), slots=4)
+    good = Request([3, 1, 4], max_tokens=5, temperature=0.8, seed=7, n=2)
+    want = dec.generate([good])[0]
+    nothing = Request([2, 2], max_tokens=5, allowed_token_ids=[9], logit_bias={9: float("-inf")}, **rule)
+    failed = {}
+    out = dec.generate([nothing, good], failed=failed)
+    assert out[1] == want and out[0] == [[]] and list(failed) == [0] and isinstance(failed[0], ValueError)
+    with pytest.raises(ValueError, match="leave no token"):
+        dec.generate([good, nothing])
+    poisoned, failed, made = Request([5, 6], max_tokens=5, n=2, **rule), {}, {}
+    for i, w, token in dec.run([poisoned, good], failed=failed):
+        made.setdefault((i, w), []).append(token)
+        page = int(dec.cache.page_table[1, 0])  # the second completion of the first request, while it is held
+        if page >= 0:
+            dec.cache.scales[0, page, 1, 0, 0] = float("nan")
+    assert [made[1, 0], made[1, 1]] == want and len(made[0, 0]) == len(made[0, 1]) == 1
+    assert list(failed) == [0] and isinstance(failed[0], RuntimeError)
+    assert int(dec.cache.ref_counts.sum()) == 0 and int(dec.cache.seq_lens.sum()) == 0
+    assert dec.generate([good])[0] == want  # the pages that were poisoned serve again
+
+
+def test_the_server_answers_the_others(tmp_path):
+    from test_transformers_model import _export
+    _export(tmp_path, {})
+    engine, server, url = _serve(tmp_path, "cpu")
+    try:
+        good = {"prompt": "w1 w2", "max_tokens": 4}
+        want = json.loads(_post(url, good)[1])["choices"]
+        bodies = [good, {"prompt": "w3", "temperature": 1.0, "allowed_token_ids": [9], "logit_bias": {"9": -1e39}}, good]
+        got = [None] * len(bodies)
+
+        def ask(i):
+            got[i] = _post(url, bodies[i])
+
+        threads = [threading.Thread(target=ask, args=(i,)) for i in range(len(bodies))]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join(timeout=120)
+        assert json.loads(got[0][1])["choices"] == json.loads(got[2][1])["choices"] == want and got[1][0] == 400
+        engine.max_batch = 1  # one at a time
+        assert _post(url, bodies[1])[0] == 400 and json.loads(_post(url, good)[1])["choices"] == want
+    finally:
+        server.shutdown()
+        server.server_close()
