@@ -137,13 +137,16 @@ class Engine:
 
     def _request(self, ids: list[int], body: dict):
         from mimir_b200.serving.paged import Request
+        bias = body.get("logit_bias") or {}
+        if not isinstance(bias, dict):
+            raise ValueError("logit_bias must map token ids to values")
         request = Request(ids, max_tokens=self._max_tokens(body), temperature=float(body.get("temperature") or 0.0),
                           top_p=float(body.get("top_p") or 1.0), n=int(body.get("n") or 1),
                           seed=None if body.get("seed") is None else int(body["seed"]),
                           presence_penalty=float(body.get("presence_penalty") or 0.0),
                           frequency_penalty=float(body.get("frequency_penalty") or 0.0),
                           repetition_penalty=float(body.get("repetition_penalty") or 1.0),
-                          logit_bias={int(k): float(v) for k, v in (body.get("logit_bias") or {}).items()},
+                          logit_bias={int(k): float(v) for k, v in bias.items()},
                           allowed_token_ids=body.get("allowed_token_ids"))
         request.check(self.model.config.vocab_size, self.model.config.max_position_embeddings)
         return request
@@ -357,6 +360,10 @@ def _handler(engine: Engine):
                 results = engine.complete_all(ids, body)
             except (KeyError, ValueError, TypeError) as exc:
                 return self._send(400, {"error": {"message": str(exc)}})
+            except ConnectionError:
+                raise  # the client has gone
+            except Exception as exc:  # the engine's: this request fails, the server goes on
+                return self._send(500, {"error": {"message": str(exc)}})
             n_in, n_out = results[0][1], sum(r[2] for r in results)
             usage = {"prompt_tokens": n_in, "completion_tokens": n_out, "total_tokens": n_in + n_out}
             base = {"id": f"cmpl-{uuid.uuid4().hex}", "created": int(time.time()), "model": engine.name,

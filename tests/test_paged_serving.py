@@ -375,3 +375,28 @@ def test_the_server_answers_the_others(tmp_path):
     finally:
         server.shutdown()
         server.server_close()
+
+
+def test_errors_get_a_response(tmp_path):
+    """A field of a wrong type is the client's error; an engine that raises is the server's, and serves on."""
+    from test_transformers_model import _export
+    _export(tmp_path, {})
+    engine, server, url = _serve(tmp_path, "cpu")
+    try:
+        good = {"prompt": "w1 w2", "max_tokens": 2}
+        want = _post(url, good)
+        for field in (dict(logit_bias=[5]), dict(logit_bias="5"), dict(allowed_token_ids=5), dict(n=[1]), dict(seed={})):
+            assert _post(url, good | field)[0] == 400, field
+        generate = engine.paged.generate
+
+        def broken(*args):
+            raise RuntimeError("out of order")
+
+        engine.paged.generate = broken
+        status, raw = _post(url, good)
+        assert status == 500 and "out of order" in json.loads(raw)["error"]["message"]
+        engine.paged.generate = generate
+        assert json.loads(_post(url, good)[1])["choices"] == json.loads(want[1])["choices"]
+    finally:
+        server.shutdown()
+        server.server_close()
