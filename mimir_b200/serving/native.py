@@ -188,24 +188,27 @@ class Engine:
         return self._finish(ids, out[0, len(ids):].tolist(), body)
 
     def stream(self, ids: list[int], body: dict):
-        """Yield decoded text pieces as they are generated, then ``(None, result)`` where result
-        is what :meth:`complete` returns (stop strings cut the text and end the stream early)."""
+        """An iterator that yields decoded text pieces as they are generated, then ``(None, result)`` where result
+        is what :meth:`complete` returns (stop strings cut the text and end the stream early).  A request that is
+        refused is refused here, before the first piece."""
         if self.paged is not None:
-            yield from self._stream_paged(ids, body)
-            return
-        from transformers import TextIteratorStreamer
+            return self._stream_paged(self._request(ids, body | {"n": 1}), body)
         temperature = float(body.get("temperature") or 0.0)
         gen = self._gen_args(self._max_tokens(body)) | dict(do_sample=temperature > 0)
         if temperature > 0:
             gen.update(temperature=temperature, top_p=float(body.get("top_p") or 1.0))
+        return self._stream_model(ids, body, gen, None if body.get("seed") is None else int(body["seed"]))
+
+    def _stream_model(self, ids: list[int], body: dict, gen: dict, seed: Optional[int]):
+        from transformers import TextIteratorStreamer
         streamer = TextIteratorStreamer(self.tokenizer, skip_prompt=True, skip_special_tokens=True)
         holder: dict = {}
 
         def run():
             try:
                 with self.lock, torch.no_grad():
-                    if body.get("seed") is not None:
-                        torch.manual_seed(int(body["seed"]))
+                    if seed is not None:
+                        torch.manual_seed(seed)
                     x = torch.tensor([ids], device=self.device)
                     holder["out"] = self.model.generate(x, attention_mask=torch.ones_like(x), streamer=streamer, **gen)
             except BaseException as exc:  # reported to the reader below
@@ -233,8 +236,7 @@ class Engine:
         result = self._finish(ids, holder["out"][0, len(ids):].tolist(), body)
         yield None, (sent, result[1], result[2], "stop" if stopped else result[3])
 
-    def _stream_paged(self, ids: list[int], body: dict):
-        request = self._request(ids, body | {"n": 1})
+    def _stream_paged(self, request, body: dict):
         stops = body.get("stop") or []
         stops = [stops] if isinstance(stops, str) else [x for x in stops if x]
         new, sent, stopped = [], "", False
@@ -252,7 +254,7 @@ class Engine:
                     sent = text
                 if stopped:
                     break
-        text, n_in, n_out, finish = self._finish(ids, new, body)
+        text, n_in, n_out, finish = self._finish(request.ids, new, body)
         if not stopped and len(text) > len(sent):
             yield text[len(sent):], None
             sent = text
@@ -400,13 +402,20 @@ def _handler(engine: Engine):
             if chat:
                 event({"id": cid, "object": kind, "created": created, "model": engine.name,
                        "choices": [{"index": 0, "delta": {"role": "assistant"}, "finish_reason": None}]})
-            for piece, result in pieces:
-                if piece is not None:
-                    event(chunk(piece))
-                else:
-                    _, n_in, n_out, finish = result
-                    event(chunk(None, finish, {"prompt_tokens": n_in, "completion_tokens": n_out,
-                                               "total_tokens": n_in + n_out}))
+            try:
+                for piece, result in pieces:
+                    if piece is not None:
+                        event(chunk(piece))
+                    else:
+                        _, n_in, n_out, finish = result
+                        event(chunk(None, finish, {"prompt_tokens": n_in, "completion_tokens": n_out,
+                                                   "total_tokens": n_in + n_out}))
+            except ConnectionError:
+                raise  # the client has gone
+            except Exception as exc:  # the status has been sent
+                return event({"error": {"message": str(exc)}})
+            finally:
+                pieces.close()
             event("[DONE]")
     return Handler
 

@@ -400,3 +400,51 @@ def test_errors_get_a_response(tmp_path):
     finally:
         server.shutdown()
         server.server_close()
+
+
+def _raw(server, body):
+    """All that the server writes for one request, as it came."""
+    import socket
+    data = json.dumps(body).encode()
+    with socket.create_connection(server.server_address[:2], timeout=60) as s:
+        s.sendall(b"POST /v1/completions HTTP/1.1\r\nHost: x\r\nConnection: close\r\nContent-Length: %d\r\n\r\n" % len(data) + data)
+        out = b""
+        while chunk := s.recv(65536):
+            out += chunk
+    return out.decode()
+
+
+@pytest.mark.parametrize("kv_cache", ["fp8", "model"])
+def test_a_refused_stream_has_one_status(tmp_path, kv_cache):
+    """What a request's check refuses is refused before the first byte of the stream; what goes wrong later is an event."""
+    from test_transformers_model import _export
+    _export(tmp_path, {})
+    from test_native_serving import _tokenizer
+    from mimir_b200.serving.native import Engine, make_server
+    _tokenizer(tmp_path)
+    engine = Engine(tmp_path, "cpu", name="tiny", max_batch=4, kv_cache=kv_cache)
+    server = make_server(engine, "127.0.0.1", 0)
+    threading.Thread(target=server.serve_forever, daemon=True).start()
+    try:
+        text = _raw(server, {"prompt": "w1", "stream": True, "temperature": "warm"})
+        assert text.startswith("HTTP/1.1 400 ") and text.count("HTTP/1.1") == 1 and "text/event-stream" not in text
+        if kv_cache == "fp8":
+            text = _raw(server, {"prompt": "w1", "stream": True, "top_p": -1})
+            assert text.startswith("HTTP/1.1 400 ") and text.count("HTTP/1.1") == 1
+        target = engine.paged if kv_cache == "fp8" else engine.model
+        name = "run" if kv_cache == "fp8" else "generate"
+
+        def broken(*args, **kw):
+            raise ValueError("out of order")
+
+        whole = getattr(target, name)
+        setattr(target, name, broken)
+        text = _raw(server, {"prompt": "w1", "stream": True})
+        assert text.startswith("HTTP/1.1 200 ") and text.count("HTTP/1.1") == 1
+        events = [line[6:] for line in text.splitlines() if line.startswith("data: ")]
+        assert "out of order" in json.loads(events[-1])["error"]["message"]
+        setattr(target, name, whole)
+        assert _raw(server, {"prompt": "w1", "stream": True, "max_tokens": 3}).rstrip().endswith("data: [DONE]")
+    finally:
+        server.shutdown()
+        server.server_close()
