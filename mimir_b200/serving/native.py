@@ -36,7 +36,9 @@ Usage: ``python -m mimir_b200.serving.native MODEL_DIR [--port 8000] [--device c
 from __future__ import annotations
 
 import argparse
+import contextlib
 import json
+import queue
 import threading
 import time
 import uuid
@@ -237,11 +239,28 @@ class Engine:
         yield None, (sent, result[1], result[2], "stop" if stopped else result[3])
 
     def _stream_paged(self, request, body: dict):
+        tokens: queue.SimpleQueue = queue.SimpleQueue()  # then None, or the exception that ended generation
+        gone = threading.Event()
+
+        def run():  # holds the lock, and waits for no reader
+            try:
+                with self.lock, contextlib.closing(self.paged.run([request], self.tokenizer.eos_token_id)) as made:
+                    for _, _, token in made:
+                        tokens.put(token)
+                        if gone.is_set():
+                            break
+                tokens.put(None)
+            except BaseException as exc:  # raised by the reader below
+                tokens.put(exc)
+
+        threading.Thread(target=run, daemon=True).start()
         stops = body.get("stop") or []
         stops = [stops] if isinstance(stops, str) else [x for x in stops if x]
         new, sent, stopped = [], "", False
-        with self.lock:
-            for _, _, token in self.paged.run([request], self.tokenizer.eos_token_id):
+        try:
+            while (token := tokens.get()) is not None:
+                if isinstance(token, BaseException):
+                    raise token
                 new.append(token)
                 text = self.tokenizer.decode(new, skip_special_tokens=True)
                 cut = min((text.find(x) for x in stops if x in text), default=-1)
@@ -254,6 +273,8 @@ class Engine:
                     sent = text
                 if stopped:
                     break
+        finally:
+            gone.set()
         text, n_in, n_out, finish = self._finish(request.ids, new, body)
         if not stopped and len(text) > len(sent):
             yield text[len(sent):], None

@@ -448,3 +448,47 @@ def test_a_refused_stream_has_one_status(tmp_path, kv_cache):
     finally:
         server.shutdown()
         server.server_close()
+
+
+def test_a_stream_that_is_not_read_stops_nobody(tmp_path):
+    """A reader takes one piece and no more: other requests and streams are answered; a reader that goes away ends
+    its generation."""
+    from test_transformers_model import _export
+    _export(tmp_path, {})
+    engine, server, url = _serve(tmp_path, "cpu")
+    try:
+        body = {"prompt": "w1 w2 w3", "max_tokens": 40, "logit_bias": {str(i): -1000 for i in range(3)}}
+        ids = engine.prompt_ids(body, False)
+        want = engine.complete(ids, body)
+        assert want[2] == 40
+        idle = engine.stream(ids, body)
+        first = next(idle)[0]
+        done = []
+        other = threading.Thread(daemon=True, target=lambda: done.append(
+            (engine.complete(ids, body), list(engine.stream(ids, body))[-1][1])))
+        other.start()
+        other.join(timeout=60)
+        assert done == [(want, want)]
+        assert first + "".join(piece for piece, _ in idle if piece is not None) == want[0]
+        # a reader that goes away after its first piece
+        steps, model = [], engine.model.model
+        forward = model.forward_paged
+        reached = threading.Event()
+
+        def counted(*args):
+            steps.append(1)
+            if len(steps) == 5:
+                reached.wait(30)
+            return forward(*args)
+
+        model.forward_paged = counted
+        gone = engine.stream(ids, body)
+        next(gone)
+        gone.close()
+        reached.set()
+        with engine.lock:
+            pass
+        assert len(steps) < 40 and int(engine.paged.cache.ref_counts.sum()) == 0
+    finally:
+        server.shutdown()
+        server.server_close()
