@@ -27,12 +27,29 @@ import math
 
 import torch
 
-from mimir_b200.ops._ext import ext, kernels_enabled
+from mimir_b200.ops._ext import KernelTimeout, available, ext, kernels_enabled
 
 BLOCK = 16       # tokens that share a scale
 MIN_EXPONENT = -32
 PAGE_SIZES = (16, 32, 64, 128, 256)
 MAX_SEQUENCES = 4096  # of one cache_reserve or cache_fork on CUDA
+
+
+def cache_status(device: torch.device) -> int:
+    """The first code that a cache kernel on ``device`` has reported since the last read (0: none).  Waits for the
+    current stream."""
+    if device.type != "cuda" or not available():
+        return 0
+    return int(ext().cache_status(device.index if device.index is not None else torch.cuda.current_device()))
+
+
+def check_cache_status(device: torch.device) -> None:
+    """Raise :class:`mimir_b200.ops._ext.KernelTimeout` where a cache kernel reported a call whose results are not
+    valid: a slot, page or length that it does not have, or a wait that ran out."""
+    code = cache_status(device)
+    if code:
+        raise KernelTimeout(f"kv_cache kernels reported code {code}: "
+                            f"{('bad slot', 'bad page', 'bad length', 'wait timed out')[min(code, 4) - 1]}")
 
 
 def _need(condition: bool, message: str) -> None:

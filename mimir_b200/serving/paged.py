@@ -21,7 +21,7 @@ from typing import Iterator, Optional
 import torch
 
 from mimir_b200 import ops
-from mimir_b200.ops.kv_cache import BLOCK, MAX_SEQUENCES
+from mimir_b200.ops.kv_cache import BLOCK, MAX_SEQUENCES, check_cache_status
 
 
 def rotary_tables(positions: int, dim: int, theta: float, device) -> tuple[torch.Tensor, torch.Tensor]:
@@ -299,6 +299,7 @@ class PagedDecoder:
                     kw["token_lens"] = cache.seq_lens[where]
                     kw["tokens"] = self.history[where, :max(len(r.ids) + made[k] for (r, _), k in zip(rows, live))]
                 tokens = self._sample(ops.process_logits(logits, **kw), rows, generators)
+                check_cache_status(self.device)  # the host has waited for the step
                 lost = {}
                 for row, ((i, _), token) in enumerate(zip(live, tokens)):
                     if token is None and not bool(torch.isfinite(logits[row]).all()):

@@ -492,3 +492,29 @@ def test_a_stream_that_is_not_read_stops_nobody(tmp_path):
     finally:
         server.shutdown()
         server.server_close()
+
+
+def test_a_kernel_report_fails_the_batch(tmp_path, monkeypatch):
+    """What the cache kernels report (here: a stand-in for it) is read in every step: no text comes of such a step."""
+    from test_transformers_model import _export
+    from mimir_b200.ops import kv_cache
+    from mimir_b200.ops._ext import KernelTimeout
+    _export(tmp_path, {})
+    engine, server, url = _serve(tmp_path, "cpu")
+    try:
+        good = {"prompt": "w1 w2", "max_tokens": 4}
+        want = json.loads(_post(url, good)[1])["choices"]
+        codes = [0, 0, 2, 0]
+        monkeypatch.setattr(kv_cache, "cache_status", lambda device: codes.pop(0) if codes else 0)
+        made = []
+        with pytest.raises(KernelTimeout, match="kv_cache"):
+            for _, _, token in engine.paged.run([Request([1, 2], max_tokens=4)]):
+                made.append(token)
+        assert len(made) == 2
+        codes[:] = [0, 1]
+        assert _post(url, good)[0] == 500
+        assert json.loads(_post(url, good)[1])["choices"] == want
+        assert int(engine.paged.cache.ref_counts.sum()) == 0
+    finally:
+        server.shutdown()
+        server.server_close()
