@@ -57,26 +57,25 @@ class PagedCache:
     def device(self):
         return self.pages.device
 
-    def _done(self, missing: torch.Tensor) -> int:
-        missing = int(missing)
-        if missing < 0:
-            raise ValueError("a sequence of the paged cache would be longer than its page table")
-        return missing
+    def _growing(self, call) -> None:
+        """``call`` returns the number of pages that lack: once more then, with as many."""
+        for again in (False, True):
+            missing = int(call())
+            if missing < 0:
+                raise ValueError("a sequence of the paged cache would be longer than its page table")
+            if missing == 0:
+                return
+            if again:
+                raise RuntimeError(f"the paged cache lacks {missing} pages after it has grown")
+            self.resize(self.pages.shape[1] + max(missing, self.pages.shape[1] // 2))
 
     def reserve(self, slots, counts) -> None:
         """Room for ``counts[i]`` more tokens of ``slots[i]``; the pool grows if its pages run out."""
-        book = (self.page_table, self.seq_lens, self.ref_counts)
-        missing = self._done(ops.cache_reserve(*book, slots, counts, self.page_size))
-        if missing:
-            self.resize(self.pages.shape[1] + max(missing, self.pages.shape[1] // 2))
-            self._done(ops.cache_reserve(self.page_table, self.seq_lens, self.ref_counts, slots, counts, self.page_size))
+        self._growing(lambda: ops.cache_reserve(self.page_table, self.seq_lens, self.ref_counts, slots, counts, self.page_size))
 
     def fork(self, src, dst) -> None:
         """``dst[i]`` becomes a copy of ``src[i]``: whole pages are shared."""
-        missing = self._done(ops.cache_fork(self.pages, self.scales, self.page_table, self.seq_lens, self.ref_counts, src, dst))
-        if missing:
-            self.resize(self.pages.shape[1] + max(missing, self.pages.shape[1] // 2))
-            ops.cache_fork(self.pages, self.scales, self.page_table, self.seq_lens, self.ref_counts, src, dst)
+        self._growing(lambda: ops.cache_fork(self.pages, self.scales, self.page_table, self.seq_lens, self.ref_counts, src, dst))
 
     def free(self, slots) -> None:
         ops.cache_free(self.page_table, self.seq_lens, self.ref_counts, slots)

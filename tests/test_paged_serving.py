@@ -518,3 +518,16 @@ def test_a_kernel_report_fails_the_batch(tmp_path, monkeypatch):
     finally:
         server.shutdown()
         server.server_close()
+
+
+@pytest.mark.parametrize("which", ["cache_reserve", "cache_fork"])
+def test_a_pool_that_still_lacks_pages_after_growing(tmp_path, monkeypatch, which):
+    """The second call's result counts as the first one's does."""
+    from mimir_b200 import ops
+    from mimir_b200.serving.paged import PagedCache
+    cache = PagedCache(1, 2, 64, 1, 8, page_size=16, pages=4)
+    cache.reserve([0], [20])
+    monkeypatch.setattr(ops, which, lambda *args: torch.ones(1, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="1 pages"):
+        cache.reserve([0], [1]) if which == "cache_reserve" else cache.fork([0], [1])
+    assert cache.pages.shape[1] > 4
