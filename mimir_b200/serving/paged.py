@@ -227,12 +227,12 @@ class PagedDecoder:
         return kw
 
     @staticmethod
-    def _sample(logits: torch.Tensor, rows: list[tuple[Request, int]], generators: dict) -> list[Optional[int]]:
+    def _sample(logits: torch.Tensor, reqs: list[Request], generators: list) -> list[Optional[int]]:
         """A token of each row; None where there is none to choose: NaN among the logits, or everything forbidden.
         (Such rows do not come to ``torch.multinomial``, which reports them by an assertion on the device.)"""
         best, good = logits.argmax(-1), logits.amax(-1) > -math.inf  # a maximum among NaN is NaN
         chances = {}
-        for i, (r, _) in enumerate(rows):
+        for i, r in enumerate(reqs):
             if r.temperature <= 0:
                 continue
             p = torch.softmax(logits[i] / r.temperature, -1)
@@ -247,8 +247,7 @@ class PagedDecoder:
         out = []
         for i, (token, ok) in enumerate(torch.stack((best, good.long()), -1).tolist()):  # one wait
             if ok and i in chances:
-                r, which = rows[i]
-                token = int(torch.multinomial(chances[i], 1, generator=generators.get((id(r), which))))
+                token = int(torch.multinomial(chances[i], 1, generator=generators[i]))
             out.append(token if ok else None)
         return out
 
@@ -269,8 +268,8 @@ class PagedDecoder:
             self._make(slots)
         cache, used = self.cache, list(range(slots))
         first = [sum(r.n for r in requests[:i]) for i in range(len(requests))]
-        generators = {(id(r), w): torch.Generator(self.device).manual_seed(r.seed + w)
-                      for r in requests if r.seed is not None for w in range(r.n)}
+        generators = {(i, w): torch.Generator(self.device).manual_seed(r.seed + w)
+                      for i, r in enumerate(requests) if r.seed is not None for w in range(r.n)}
         try:
             # ---- prompts, packed; then a slot for each further completion
             counts = [len(r.ids) for r in requests]
@@ -297,7 +296,7 @@ class PagedDecoder:
                     where = torch.tensor(at, device=self.device)
                     kw["token_lens"] = cache.seq_lens[where]
                     kw["tokens"] = self.history[where, :max(len(r.ids) + made[k] for (r, _), k in zip(rows, live))]
-                tokens = self._sample(ops.process_logits(logits, **kw), rows, generators)
+                tokens = self._sample(ops.process_logits(logits, **kw), [r for r, _ in rows], [generators.get(k) for k in live])
                 check_cache_status(self.device)  # the host has waited for the step
                 lost = {}
                 for row, ((i, _), token) in enumerate(zip(live, tokens)):

@@ -531,3 +531,11 @@ def test_a_pool_that_still_lacks_pages_after_growing(tmp_path, monkeypatch, whic
     with pytest.raises(RuntimeError, match="1 pages"):
         cache.reserve([0], [1]) if which == "cache_reserve" else cache.fork([0], [1])
     assert cache.pages.shape[1] > 4
+
+
+def test_one_request_object_twice_in_a_batch(tmp_path):
+    """Equal requests get equal completions, the same object or not."""
+    dec = PagedDecoder(_model(tmp_path), slots=4)
+    r = Request([4, 2], max_tokens=8, temperature=1.0, seed=3)
+    want = dec.generate([r])[0]
+    assert dec.generate([r, r]) == [want, want]
