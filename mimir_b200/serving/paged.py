@@ -189,6 +189,7 @@ class PagedDecoder:
         self.model, self.config, self.device = model, cfg, device
         self.layers = cfg.num_layers_per_stack * cfg.H_cycles * (cfg.L_cycles + 1)
         self.page_size, self.pages = page_size, pages
+        self._running = False
         self._make(slots)
 
     def _make(self, slots: int) -> None:
@@ -264,12 +265,15 @@ class PagedDecoder:
         slots = sum(r.n for r in requests)
         if slots > MAX_SEQUENCES:
             raise ValueError(f"{slots} completions side by side are more than {MAX_SEQUENCES}")
+        if self._running:
+            raise RuntimeError("a batch of this decoder is not finished (nor closed): it holds the slots")
         if slots > self.cache.page_table.shape[0]:
             self._make(slots)
         cache, used = self.cache, list(range(slots))
         first = [sum(r.n for r in requests[:i]) for i in range(len(requests))]
         generators = {(i, w): torch.Generator(self.device).manual_seed(r.seed + w)
                       for i, r in enumerate(requests) if r.seed is not None for w in range(r.n)}
+        self._running = True
         try:
             # ---- prompts, packed; then a slot for each further completion
             counts = [len(r.ids) for r in requests]
@@ -334,6 +338,7 @@ class PagedDecoder:
                 batch.ngram_history, batch.ngram_lens = self.history, lens
                 logits = self.model.lm_head(self.model.model.forward_paged(ids.to(self.device, torch.long), batch))
         finally:
+            self._running = False
             if used:
                 cache.free(used)
 

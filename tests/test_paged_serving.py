@@ -539,3 +539,18 @@ def test_one_request_object_twice_in_a_batch(tmp_path):
     r = Request([4, 2], max_tokens=8, temperature=1.0, seed=3)
     want = dec.generate([r])[0]
     assert dec.generate([r, r]) == [want, want]
+
+
+def test_one_batch_at_a_time(tmp_path):
+    """A second batch beside one that is not finished would take the same slots: it is refused."""
+    dec = PagedDecoder(_model(tmp_path), slots=2)
+    want = dec.generate([Request([1, 2], max_tokens=6)])[0][0]
+    made = dec.run([Request([1, 2], max_tokens=6)])
+    tokens = [next(made)[2]]
+    with pytest.raises(RuntimeError, match="not finished"):
+        dec.generate([Request([3], max_tokens=2)])
+    assert tokens + [t for _, _, t in made] == want
+    made = dec.run([Request([1, 2], max_tokens=6)])
+    next(made)
+    made.close()
+    assert dec.generate([Request([1, 2], max_tokens=6)])[0][0] == want
