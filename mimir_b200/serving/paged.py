@@ -21,7 +21,8 @@ from typing import Iterator, Optional
 import torch
 
 from mimir_b200 import ops
-from mimir_b200.ops.kv_cache import BLOCK, MAX_SEQUENCES, check_cache_status
+from mimir_b200.ops._ext import KernelTimeout
+from mimir_b200.ops.kv_cache import BLOCK, MAX_SEQUENCES, cache_status, check_cache_status
 
 
 def rotary_tables(positions: int, dim: int, theta: float, device) -> tuple[torch.Tensor, torch.Tensor]:
@@ -273,7 +274,7 @@ class PagedDecoder:
         first = [sum(r.n for r in requests[:i]) for i in range(len(requests))]
         generators = {(i, w): torch.Generator(self.device).manual_seed(r.seed + w)
                       for i, r in enumerate(requests) if r.seed is not None for w in range(r.n)}
-        self._running = True
+        self._running, reported = True, False
         try:
             # ---- prompts, packed; then a slot for each further completion
             counts = [len(r.ids) for r in requests]
@@ -337,10 +338,15 @@ class PagedDecoder:
                 batch = cache.batch(at, [1] * len(at))
                 batch.ngram_history, batch.ngram_lens = self.history, lens
                 logits = self.model.lm_head(self.model.model.forward_paged(ids.to(self.device, torch.long), batch))
+        except KernelTimeout:
+            reported = True
+            raise
         finally:
             self._running = False
             if used:
                 cache.free(used)
+            if reported:
+                cache_status(self.device)  # what freeing a bad page reports is this batch's too, not the next one's
 
     def generate(self, requests: list[Request], eos: Optional[int] = None,
                  failed: Optional[dict] = None) -> list[list[list[int]]]:

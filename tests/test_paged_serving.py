@@ -554,3 +554,37 @@ def test_one_batch_at_a_time(tmp_path):
     next(made)
     made.close()
     assert dec.generate([Request([1, 2], max_tokens=6)])[0][0] == want
+
+
+@pytest.mark.gpu
+@torch.no_grad()
+@pytest.mark.parametrize("rule", [dict(temperature=0.9, seed=1), dict()], ids=["sampled", "greedy"])
+def test_a_request_without_a_token_to_choose_fails_alone_on_the_gpu(tmp_path, rule):
+    dec = PagedDecoder(_model(tmp_path, GPU, "cuda", torch.bfloat16), slots=4)
+    good = Request([3, 1, 4], max_tokens=5, temperature=0.8, seed=7, n=2)
+    want = dec.generate([good])[0]
+    nothing = Request([2, 2], max_tokens=5, allowed_token_ids=[9], logit_bias={9: float("-inf")}, **rule)
+    poisoned, failed, lengths = Request([5, 6], max_tokens=5, **rule), {}, [0, 0, 0]
+    for i, _, _ in dec.run([nothing, poisoned, good], failed=failed):
+        lengths[i] += 1
+        page = int(dec.cache.page_table[1, 0])
+        if page >= 0:
+            dec.cache.scales[0, page, 1, 0, 0] = float("nan")
+    assert lengths == [0, 1, 10] and isinstance(failed[0], ValueError) and isinstance(failed[1], RuntimeError)
+    assert dec.generate([good])[0] == want
+
+
+@pytest.mark.gpu
+@torch.no_grad()
+def test_a_bad_page_fails_the_batch_on_the_gpu(tmp_path):
+    from mimir_b200.ops._ext import KernelTimeout
+    dec = PagedDecoder(_model(tmp_path, GPU, "cuda", torch.bfloat16), slots=2)
+    want = dec.generate([Request([3, 1], max_tokens=4)])[0]
+    made = dec.run([Request([3, 1], max_tokens=4)])
+    next(made)
+    page = int(dec.cache.page_table[0, 0])
+    dec.cache.page_table[0, 0] = 10 ** 6  # skipped and reported
+    with pytest.raises(KernelTimeout, match="bad page"):
+        next(made)
+    dec.cache.ref_counts[page] = 0
+    assert dec.generate([Request([3, 1], max_tokens=4)])[0] == want
