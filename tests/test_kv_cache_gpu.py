@@ -704,3 +704,80 @@ def test_graphs_leave_little_memory_behind():
     torch.cuda.synchronize()
     torch.cuda.empty_cache()
     assert torch.cuda.memory_reserved() - before <= 2 * 2 ** 20
+
+
+def test_streams_and_graphs_side_by_side():
+    """Workspaces are a stream's or a graph's own: what runs at once does not mix."""
+    sizes = ([9000, 40, 3000], [700] * 20, [20000])
+    sets = [filled(lens, 2, 64, seed=i) for i, lens in enumerate(sizes)]
+    calls = []
+    for st, lens in zip(sets, sizes):
+        n = len(lens)
+        q = torch.randn(n, 8, DIM, device=DEV, generator=torch.Generator(DEV).manual_seed(n)).bfloat16()
+        args = (q, st["pages"], st["scales"], st["table"], st["lens"], ints(list(range(n))).to(DEV), ints(list(range(n + 1))).to(DEV))
+        calls.append((lambda a=args: ops.cache_attention(*a, max_new=1)))
+    want = [call() for call in calls]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = calls[0]()
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(3):
+        torch.cuda.synchronize()
+        got = [[] for _ in calls]
+        for _ in range(10):
+            graph.replay()
+            for stream, call, out in zip(streams, calls, got):
+                with torch.cuda.stream(stream):
+                    out.append(call())
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want[0])
+        for outs, w in zip(got, want):
+            assert all(torch.equal(o, w) for o in outs)
+    check_kernel_status(DEV)
+
+
+@pytest.mark.parametrize("kernel", [1, 2])
+def test_attention_of_several_tokens_in_a_graph(kernel):
+    st = filled([600, 700], 2, 64)
+    q = torch.randn(100, 8, DIM, device=DEV).bfloat16()
+    cu, seqs = ints([0, 40, 90]).to(DEV), ints([0, 1]).to(DEV)
+    call = lambda: ext().cache_attention(q, st["pages"], st["scales"], st["table"], st["lens"], seqs, cu, None,  # noqa: E731
+                                         DIM ** -0.5, 0, kernel)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for lens, bounds in (([600, 700], [0, 40, 90]), ([64, 99], [0, 1, 100]), ([500, 3], [0, 97, 100])):
+        st["lens"].copy_(ints(lens))
+        cu.copy_(ints(bounds))
+        q.copy_(torch.randn(100, 8, DIM))
+        graph.replay()
+        assert torch.equal(out, call())
+    check_kernel_status(DEV)
+
+
+def test_prompts_do_not_depend_on_the_run():
+    counts = [700, 33, 2000]
+    st = filled(counts, 4, 64)
+    q, first = check_attention(st, [0, 1, 2], counts, 16, prefix=[700, 0, 1000], kernel=2)
+    for _ in range(5):
+        assert torch.equal(attend(q, st, [0, 1, 2], [0, 700, 733, 2733], [700, 0, 1000], kernel=2), first)
+
+
+def test_compaction_into_a_pool_that_is_too_small():
+    st = {k: t.to(DEV) for k, t in pool(12, 1, 16, DIM, 4, 3, layers=2).items()}
+    book = (st["table"], st["lens"], st["refs"])
+    ops.cache_reserve(*book, [0, 1, 2], [40, 17, 33], 16)
+    ops.cache_free(*book, [1])
+
+    def other(pages):
+        return (torch.zeros(2, pages, 2, 1, 16, DIM, device=DEV).to(torch.float8_e4m3fn), torch.zeros(2, pages, 2, 1, 1, device=DEV),
+                torch.full_like(st["table"], 77), ints([9] * pages).to(DEV))
+
+    small, fits = other(5), other(6)
+    assert ops.cache_compact(st["pages"], st["scales"], st["table"], st["refs"], small).item() == 1
+    assert not small[0].view(torch.uint8).any() and not small[1].any() and (small[2] == 77).all() and (small[3] == 9).all()
+    assert ops.cache_compact(st["pages"], st["scales"], st["table"], st["refs"], fits).item() == 0
+    assert fits[2].tolist() == [[0, 1, 2, -1], [-1] * 4, [5, 3, 4, -1]] and fits[3].tolist() == [1] * 6
+    check_kernel_status(DEV)
