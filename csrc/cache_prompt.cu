@@ -62,7 +62,7 @@ struct __align__(8) Barriers {
   uint64_t k_full[2], v_full[2]; // converted
   uint64_t k_empty[2], v_empty[2];
   uint64_t s_full[2][2], p_full[2][2];  // per row tile and buffer
-  uint64_t o_done[2];                   // per row tile
+  uint64_t o_done[2][2];                // the same, of products
   uint64_t mma_done;
   uint32_t tmem_base;
   int pad;
@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int i = 0; i < 2; ++i) {
         mbar_init(&bar->s_full[s][i], 1);
         mbar_init(&bar->p_full[s][i], 4);
+        mbar_init(&bar->o_done[s][i], 1);
       }
-      mbar_init(&bar->o_done[s], 1);
     }
     for (int s = 0; s < kScaleRing; ++s) mbar_init(&bar->scales_full[s], 16);
     mbar_init(&bar->mma_done, 2);
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < 4; ++k)  // 16 keys: 8 packed columns of P, 2 KB of V
           mma_ts(d, a + k * 8, b + k * (2048 >> 4), idesc_pv, (i > 0 || k > 0) ? 1u : 0u, leader);
-        commit(&bar->o_done[x]);
+        commit(&bar->o_done[x][i & 1]);
       };
       int k_seen = -1, v_seen = -1;  // tiles whose keys and values are known to have come
       auto keys_ready = [&](int tile) {
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if ((i + 1) * kHalf > min_lim) probabilities(std::true_type{});
       else probabilities(std::false_type{});
       if (__any_sync(0xffffffff, rescale)) {  // O is touched: its last product has to be done
-        ok = warp_wait(&bar->o_done[x], (i - 1) & 1, status, kCacheTimeout);
+        ok = warp_wait(&bar->o_done[x][(i - 1) & 1], (i - 1) >> 1 & 1, status, kCacheTimeout);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll
@@ -627,9 +627,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar->p_full[x][i & 1]);
     }
-    // The last S came after all products but two: wait for either, since a parity tells only neighbours apart.
-    if (ok && my_turns > 1) ok = warp_wait(&bar->o_done[x], (my_turns - 2) & 1, status, kCacheTimeout);
-    if (ok && my_turns > 0) ok = warp_wait(&bar->o_done[x], (my_turns - 1) & 1, status, kCacheTimeout);
+    // A parity tells only neighbouring phases apart.  Of the last two products either may be done by now, so they have
+    // a barrier each (with one for both, the wait for the first would miss its phase when the second is done too); all
+    // before them were done when the last scores came.
+    for (int i = max(my_turns - 2, 0); ok && i < my_turns; ++i)
+      ok = warp_wait(&bar->o_done[x][i & 1], i >> 1 & 1, status, kCacheTimeout);
     tc_fence_after();
     const float inv_l = l > 0.f || l != l ? 1.f / l : 0.f;
     uint4* dst = reinterpret_cast<uint4*>(p.out) + ((int64_t)(first_row + tok) * p.H + kvh * group + r % group) * (kCacheDim / 8);
