@@ -264,6 +264,8 @@ class PagedDecoder:
         for r in requests:
             r.check(vocab, limit)
         slots = sum(r.n for r in requests)
+        if not requests:
+            return
         if slots > MAX_SEQUENCES:
             raise ValueError(f"{slots} completions side by side are more than {MAX_SEQUENCES}")
         if self._running:

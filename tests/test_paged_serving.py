@@ -588,3 +588,7 @@ def test_a_bad_page_fails_the_batch_on_the_gpu(tmp_path):
         next(made)
     dec.cache.ref_counts[page] = 0
     assert dec.generate([Request([3, 1], max_tokens=4)])[0] == want
+
+
+def test_no_requests_give_no_completions(tmp_path):
+    assert PagedDecoder(_model(tmp_path), slots=2).generate([]) == []
