@@ -232,25 +232,21 @@ class PagedDecoder:
     def _sample(logits: torch.Tensor, reqs: list[Request], generators: list) -> list[Optional[int]]:
         """A token of each row; None where there is none to choose: NaN among the logits, or everything forbidden.
         (Such rows do not come to ``torch.multinomial``, which reports them by an assertion on the device.)"""
-        best, good = logits.argmax(-1), logits.amax(-1) > -math.inf  # a maximum among NaN is NaN
-        chances = {}
-        for i, r in enumerate(reqs):
+        best = logits.max(-1)  # NaN where one is among them; of equal ones the first
+        out = []
+        for i, (r, top, token) in enumerate(zip(reqs, *torch.stack((best.values.double(), best.indices.double())).tolist())):
             if r.temperature <= 0:
+                out.append(int(token) if top > -math.inf else None)
+                continue
+            if not abs(top / r.temperature) < FLOAT32_MAX:  # softmax is finite where its largest argument is
+                out.append(None)
                 continue
             p = torch.softmax(logits[i] / r.temperature, -1)
             if r.top_p < 1.0:
                 order = p.argsort(descending=True, stable=True)
                 ahead = p[order].cumsum(-1) - p[order]
                 p = p.index_fill(0, order[ahead >= r.top_p], 0.0)
-            chances[i] = p
-        if chances:
-            sums = torch.stack([p.sum() for p in chances.values()])
-            good[list(chances)] &= (sums > 0) & (sums < math.inf)
-        out = []
-        for i, (token, ok) in enumerate(torch.stack((best, good.long()), -1).tolist()):  # one wait
-            if ok and i in chances:
-                token = int(torch.multinomial(chances[i], 1, generator=generators[i]))
-            out.append(token if ok else None)
+            out.append(int(torch.multinomial(p, 1, generator=generators[i])))
         return out
 
     @torch.no_grad()
