@@ -18,16 +18,17 @@
 // query rows as the 8 columns: a group's few rows fill the narrow side.  Bytes become fp16
 // exactly; the scales, powers of two, stay outside: a key block's multiplies its scores, a value
 // block's enters the exponent of the probability that multiplies the values, exp2(x + ev - M) with a
-// maximum M of x + ev of its own (so it neither overflows nor loses small weights), beside exp2(x - m)
-// for the sum.  Probabilities are rounded to fp16 (11 bits) for the product.  Query rows are shifted by
-// a power of two into fp16's range, so that bf16 rows keep all their bits.
+// maximum M of x + ev of its own, beside exp2(x - m) for the sum.  Probabilities are rounded to fp16 for the
+// product: to 11 bits, and below 2^-14 to 2^-25 of the largest product of weight and value scale.  Query rows are
+// shifted by a power of two into fp16's range: bf16 values keep all their bits down to 2^-27 of the row's largest,
+// smaller ones are rounded to 2^-38 of it.
 // The contraction over the head dimension may run in any order: thread c of a quad takes the bytes
 // 32c..32c+31 of a key row, which two 16-byte loads bring without bank conflicts under the swizzle, and
 // the same dimensions of the query rows.  Of the values thread (g, c) takes the bytes 16g..16g+15 of
 // four rows; row g of product j is dimension 16g + 2j, row g + 8 the one after it.
 //
-// Measured on B200 (16 query and 4 key/value heads, one new token): 64 sequences to 8000 tokens 40 us for
-// 166 MB; 8 sequences to 100001 tokens 74 us for 391 MB (5.3 TB/s; 6.4 TB/s between two lengths, where the
+// Measured on B200 (16 query and 4 key/value heads, one new token): 64 sequences to 8000 tokens 41 us for
+// 166 MB; 8 sequences to 100001 tokens 75 us for 391 MB (5.2 TB/s; 6.4 TB/s between two lengths, where the
 // some 10 us of start and joining cancel); DRAM reads are the cache's bytes and no more.  24 sequences to
 // 2100 tokens, 7 tokens, 20 and 20 heads: 44 us for 138 MB.  With the rows as the wide side of the products
 // (half of it empty) a warp needs 406 instructions for 16 keys instead of some 200: 55, 87 and 83 us.
@@ -466,7 +467,7 @@ __global__ void __launch_bounds__(kThreads, Shape<kTiles>::kBlocksPerSm) cache_a
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // the row's largest value to [2^13, 2^14): a power of two, nothing is rounded away
+      // the row's largest value to [2^13, 2^14): what is not under 2^-27 of it keeps its bits
       const int shift = max(min(13 - ((__float_as_int(top) >> 23) - 127), 120), -115);
       const float f = __int_as_float((shift + 127) << 23);
 #pragma unroll

@@ -16,16 +16,17 @@
 //
 // The scales, powers of two of 16 keys each, stay outside the products: a key block's multiplies its
 // scores, a value block's enters the exponent, p = exp2(x + ev - M) with M the maximum of x + ev, so that
-// p <= 1 is rounded to fp16 beside the largest product of weight and value scale; the sum of the weights
-// takes each block's sum times 2^-ev in fp32.  Query rows are shifted by a power of two into fp16's
-// range first, so that bf16 rows keep all their bits.
+// p <= 2^8 (M lags by as much) is rounded to fp16 beside the largest product of weight and value scale; the
+// sum of the weights takes each block's sum times 2^-ev in fp32.  Query rows are shifted by a power of two
+// into fp16's range first: bf16 values keep all their bits down to 2^-27 of the row's largest.
 //
 // TMEM (512 columns): S_X0 and S_X1, 64 columns each, for tiles A and B, then O_A and O_B, 128 each; P is
 // packed fp16 in the first 32 columns of its S and read from there as the A operand.  With one S of
 // 128 keys a tile (the same columns), scores to P to products is a chain that leaves the tensor
 // cores idle for more than half of the time; with two of 64 the next scores are there when a softmax ends.
 // Measured on B200: five prompts to 4096 tokens (13703 in all), 16 and 4 heads, every token sees its whole
-// prompt: 392 us, 876 TFLOP/s of 1641; tensor pipe active 39 % under the profiler (430 us there).  What
+// prompt: 393 us by itself, 873 TFLOP/s of 1641, and 407 us, 844 TFLOP/s, between other work at the clocks that it
+// leaves; tensor pipe active 39 % under the profiler (430 us there).  What
 // bounds it: the products with next to nothing between them take 350 us, the softmax with half of the
 // products 401 (both before the order of blocks below, 416).  One S of 128 keys a tile: 489 us; one MMA warp
 // for both tiles: 478 us, since issuing takes as long as the products; a row's softmax on two warps: 473 us.
