@@ -129,7 +129,7 @@ class Batch:
 
 
 FLOAT32_MAX = torch.finfo(torch.float32).max
-LEAST_TEMPERATURE = 1e-30  # logits divided by it stay in float32
+LEAST = 1e-30              # temperature (logits divided by it stay in float32) and top_p (not rounded to zero)
 MAX_COMPLETIONS = 128      # of one request, and of a server's batch: each takes a slot of the cache
 
 
@@ -158,10 +158,10 @@ class Request:
         if self.n > MAX_COMPLETIONS:
             raise ValueError(f"n is at most {MAX_COMPLETIONS}")
         # (comparisons that NaN does not pass)
-        if not -FLOAT32_MAX <= self.temperature <= FLOAT32_MAX or 0 < self.temperature < LEAST_TEMPERATURE:
-            raise ValueError(f"temperature must be zero (greedy) or at least {LEAST_TEMPERATURE}, and finite")
-        if not self.top_p > 0:
-            raise ValueError("top_p must be positive")
+        if not -FLOAT32_MAX <= self.temperature <= FLOAT32_MAX or 0 < self.temperature < LEAST:
+            raise ValueError(f"temperature must be zero (greedy) or at least {LEAST}, and finite")
+        if not self.top_p >= LEAST:
+            raise ValueError(f"top_p must be at least {LEAST}")
         if not 2.0 ** -126 <= self.repetition_penalty <= 2.0 ** 126:
             raise ValueError("repetition_penalty and its inverse must be float32 numbers")
         if not all(abs(x) <= FLOAT32_MAX for x in (self.presence_penalty, self.frequency_penalty)):
@@ -238,7 +238,7 @@ class PagedDecoder:
             if r.temperature <= 0:
                 out.append(int(token) if top > -math.inf else None)
                 continue
-            if not abs(top / r.temperature) < FLOAT32_MAX:  # softmax is finite where its largest argument is
+            if not abs(top / r.temperature) < 2.0 ** 127:  # softmax is finite where its largest argument is
                 out.append(None)
                 continue
             p = torch.softmax(logits[i] / r.temperature, -1)

@@ -592,3 +592,12 @@ def test_a_bad_page_fails_the_batch_on_the_gpu(tmp_path):
 
 def test_no_requests_give_no_completions(tmp_path):
     assert PagedDecoder(_model(tmp_path), slots=2).generate([]) == []
+
+
+def test_rules_that_float32_rounds_to_nothing(tmp_path):
+    """A top_p that is zero in float32 keeps no token; a logit that a temperature takes to the edge of float32 may."""
+    with pytest.raises(ValueError, match="top_p"):
+        Request([1, 2], temperature=1.0, top_p=1e-320).check(96, 64)
+    logits = torch.tensor([[1.0, 3.4e8, 2.0], [1.0, 1e8, 2.0]])
+    reqs = [Request([1], temperature=1e-30, seed=1)] * 2
+    assert PagedDecoder._sample(logits, reqs, [None, None]) == [None, 1]
